@@ -324,6 +324,44 @@ RMLX_API rmlx_status rmlx_kv_append(rmlx_kv_pool* p, int32_t layer_begin, int32_
                            int64_t layer_stride, int64_t token_stride, int64_t head_stride,
                            const int32_t* slot_mapping, int32_t num_tokens, void* stream);
 
+/* Rotary position embedding of one model: pair i of a row (i < rotary_dim / 2)
+ * turns by positions[axis][token] * inv_freq[i] radians, axis = pair_axis[i]
+ * (0 when pair_axis is NULL).  Text has one axis; images and video have
+ * several (time, height, width), each owning some of the pairs.  The pair is
+ * elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; elements
+ * from rotary_dim on pass through.  Arrays are device arrays. */
+typedef struct rmlx_rope {
+  const float* inv_freq;    /* rotary_dim / 2 frequencies, radians per position */
+  const int32_t* pair_axis; /* rotary_dim / 2 axis numbers, or NULL */
+  int32_t rotary_dim;       /* a multiple of 16, at most head_dim and 1024 */
+  int32_t interleaved;
+  int32_t num_axes;         /* at least 1 */
+} rmlx_rope;
+
+/* Append with the position rotation applied on the way, for one layer: the
+ * query and key rows of `num_tokens` tokens are rotated and the key and value
+ * rows written to their slots (as rmlx_kv_append) in one launch.  No
+ * counterpart in the reference crate, whose model rotates inside the external
+ * rmlx-nn forward before the cache sees the rows (transformer.rs:125-129).
+ * Token t stands at positions[axis * position_axis_stride + t].  Row (t, h) of
+ * q starts at element t * q_token_stride + h * q_head_stride, of q_out and of
+ * k / v likewise (element type = cfg.dtype; pointers and strides multiples of
+ * 16 bytes), so rows inside one fused projection are read in place; q_out may
+ * be q with q's strides, and must not overlap q in any other way.  q_heads = 0
+ * rotates keys only.  Every token's query rows are written; a negative slot
+ * skips the token's K and V.  Slots named twice in one call leave either
+ * token's row (or a mixture of their bytes).  Angles are reduced in f64 and
+ * the rotation done in f32, rounded once to the pool's type; a quantised pool
+ * quantises the f32 rows, with no rounding between.  head_dim must be a
+ * multiple of 8.  A pair_axis entry outside [0, num_axes) is flagged
+ * (rmlx_kv_pool_check bit 8) and taken as axis 0. */
+RMLX_API rmlx_status rmlx_kv_append_rope(rmlx_kv_pool* p, int32_t layer, const rmlx_rope* rope,
+                                         const int32_t* positions, int64_t position_axis_stride, const void* q,
+                                         int32_t q_heads, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                                         int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,
+                                         const void* v, int64_t token_stride, int64_t head_stride,
+                                         const int32_t* slot_mapping, int32_t num_tokens, void* stream);
+
 /* Gather -- RotatingKVCache::get_logical_order (rotating_cache.rs:162-197)
  * over block tables.  For sequence s with length seq_lens[s], writes
  * out[(cu[s] * heads + h * seq_lens[s] + t) * head_dim ...] for every head h
@@ -377,6 +415,35 @@ RMLX_API rmlx_status rmlx_kv_decode_attention(rmlx_kv_pool* p, int32_t layer, co
                                               const int32_t* block_tables, int32_t block_table_stride,
                                               const int32_t* seq_lens, int32_t num_seqs, float softmax_scale, void* out,
                                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Chunk attention: rmlx_kv_decode_attention for any number of new tokens per
+ * sequence (prefill, chunked prefill over a cached prefix, verification of
+ * drafted tokens), the chunk's own rows already appended.  Sequence s has
+ * seq_lens[s] rows, the last q_lens[s] of them its chunk; chunk token i
+ * stands at position p = seq_lens[s] - q_lens[s] + i and sees rows j <= p,
+ * with window > 0 only j > p - window.  A token that sees no row (p < 0) gives
+ * zeros; masked rows have no influence whatever they hold.  Sequences of
+ * length 0 in q_lens take no rows of q.
+ * q: rows of all chunks back to back, num_q_tokens of them at least; row
+ * (token, query head) at element token * q_token_stride + head *
+ * q_head_stride.  out: [token][num_kv_heads * q_heads_per_kv][head_dim] in the
+ * pool's type; rows behind the last chunk are left as they were.  When q_lens
+ * sum to more than num_q_tokens the launch is flagged (rmlx_kv_pool_check bit
+ * 16) and writes nothing.  Block ids outside the pool, and rows past
+ * block_table_stride blocks, are flagged (bit 2); what their sequence's out
+ * rows then hold is unspecified.
+ * Pools, head_dim and q_heads_per_kv as for rmlx_kv_decode_attention; any
+ * block size.  A quantised pool's rows count as code * scale + zero, without
+ * the gather's rounding to cfg.dtype.  workspace: rmlx_kv_chunk_attention_workspace_size bytes, not
+ * shared by launches that may overlap. */
+RMLX_API rmlx_status rmlx_kv_chunk_attention_workspace_size(const rmlx_kv_pool* p, int32_t q_heads_per_kv,
+                                                            size_t* bytes);
+RMLX_API rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* q, int64_t q_token_stride,
+                                             int64_t q_head_stride, int32_t q_heads_per_kv,
+                                             const int32_t* block_tables, int32_t block_table_stride,
+                                             const int32_t* q_lens, const int32_t* seq_lens, int32_t num_seqs,
+                                             int32_t num_q_tokens, float softmax_scale, int32_t window, void* out,
+                                             void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- Batch block tables (the scheduler's KV bookkeeping) -----------------
  * Replaces the per-sequence KVCache / BatchKVCache slots of the scheduler

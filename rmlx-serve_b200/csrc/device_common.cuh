@@ -17,6 +17,8 @@ enum : int32_t {
   DEV_ERR_SLOT = 1,   // slot_mapping entry >= num_blocks * block_size
   DEV_ERR_BLOCK = 2,  // block-table / copy id outside [0, num_blocks)
   DEV_ERR_WORKSPACE = 4,  // a launch's splits exceed the workspace it was given
+  DEV_ERR_AXIS = 8,       // pair_axis entry outside [0, num_axes)
+  DEV_ERR_Q_ROWS = 16,    // q_lens sum past the num_q_tokens rows of a launch
 };
 
 // 16-byte streaming load through the non-coherent path without L1

@@ -159,6 +159,18 @@ _sig("rmlx_kv_gather_layers", st, vp, C.c_int32, C.c_int32, vp, C.c_int32, vp, C
 _sig("rmlx_kv_attention_workspace_size", st, vp, C.c_int32, C.c_int32, C.c_int64, C.POINTER(C.c_size_t))
 _sig("rmlx_kv_decode_attention", st, vp, C.c_int32, vp, C.c_int32, vp, C.c_int32, vp, C.c_int32, C.c_float, vp, vp,
      C.c_size_t, vp)
+
+
+class RopeStruct(C.Structure):
+    _fields_ = [("inv_freq", vp), ("pair_axis", vp), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32),
+                ("num_axes", C.c_int32)]
+
+
+_sig("rmlx_kv_append_rope", st, vp, C.c_int32, C.POINTER(RopeStruct), vp, C.c_int64, vp, C.c_int32, C.c_int64, C.c_int64,
+     vp, C.c_int64, C.c_int64, vp, vp, C.c_int64, C.c_int64, vp, C.c_int32, vp)
+_sig("rmlx_kv_chunk_attention_workspace_size", st, vp, C.c_int32, C.POINTER(C.c_size_t))
+_sig("rmlx_kv_chunk_attention", st, vp, C.c_int32, vp, C.c_int64, C.c_int64, C.c_int32, vp, C.c_int32, vp, vp, C.c_int32,
+     C.c_int32, C.c_float, C.c_int32, vp, vp, C.c_size_t, vp)
 _sig("rmlx_kv_copy_blocks", st, vp, vp, vp, C.c_int32, vp)
 
 # RotatingKVCache state over a block manager

@@ -43,6 +43,23 @@ class PoolLayout:
     meta_row_bytes: int
 
 
+class Rope:
+    """A model's rotary position embedding: pair i turns by
+    positions[pair_axis[i]] * inv_freq[i] radians.  `inv_freq` (f32) and
+    `pair_axis` (int32, None = one axis) are device arrays of
+    rotary_dim / 2 entries; the object keeps them alive."""
+
+    def __init__(self, inv_freq, rotary_dim: int, interleaved: bool = False, pair_axis=None, num_axes: int = 1):
+        for name, a, kind in (("inv_freq", inv_freq, "float32"), ("pair_axis", pair_axis, "int32")):
+            if a is None or isinstance(a, int):
+                continue
+            if str(a.dtype).split(".")[-1] != kind or a.numel() != rotary_dim // 2 or not a.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {kind} array of rotary_dim / 2 = {rotary_dim // 2} entries")
+        self.inv_freq, self.pair_axis = inv_freq, pair_axis
+        self.rotary_dim, self.interleaved, self.num_axes = rotary_dim, bool(interleaved), num_axes
+        self._c = _lib.RopeStruct(_ptr(inv_freq), _ptr(pair_axis), rotary_dim, int(self.interleaved), num_axes)
+
+
 class KVPool:
     """Block-major paged KV pool on one GPU: pool[block][layer][kv][head][slot][row]."""
 
@@ -115,6 +132,30 @@ class KVPool:
         check(lib.rmlx_kv_append(self._h, layer_begin, nl, _ptr(k), _ptr(v), ls, ts, hs, _ptr(slot_mapping),
                                  num_tokens, _stream(stream, self.device)))
 
+    def append_rope(self, layer: int, k, v, slot_mapping, num_tokens: int, positions, rope: Rope, q=None, q_out=None,
+                    q_heads: int = 0, token_stride: Optional[int] = None, head_stride: Optional[int] = None,
+                    q_token_stride: Optional[int] = None, q_head_stride: Optional[int] = None,
+                    q_out_token_stride: Optional[int] = None, q_out_head_stride: Optional[int] = None,
+                    position_axis_stride: Optional[int] = None, stream=None) -> None:
+        """Rotate the query rows of `q` into `q_out` and append the rotated
+        key rows and the value rows to their slots of one layer.
+
+        Strides are in elements and default to contiguous [tokens][heads]
+        [head_dim]; positions are int32 [num_axes][num_tokens].  `q_out` may
+        be `q` itself (with q's strides)."""
+        c = self.cfg
+        dim = c.head_dim
+        hs = dim if head_stride is None else head_stride
+        ts = c.num_kv_heads * dim if token_stride is None else token_stride
+        qhs = dim if q_head_stride is None else q_head_stride
+        qts = q_heads * dim if q_token_stride is None else q_token_stride
+        ohs = dim if q_out_head_stride is None else q_out_head_stride
+        ots = q_heads * dim if q_out_token_stride is None else q_out_token_stride
+        ps = num_tokens if position_axis_stride is None else position_axis_stride
+        check(lib.rmlx_kv_append_rope(self._h, layer, C.byref(rope._c), _ptr(positions), ps, _ptr(q), q_heads, qts, qhs,
+                                      _ptr(q_out), ots, ohs, _ptr(k), _ptr(v), ts, hs, _ptr(slot_mapping), num_tokens,
+                                      _stream(stream, self.device)))
+
     def gather(self, layer: int, block_tables, block_table_stride: int, seq_lens, num_seqs: int, out_k, out_v,
                stream=None) -> None:
         check(lib.rmlx_kv_gather(self._h, layer, _ptr(block_tables), block_table_stride, _ptr(seq_lens),
@@ -143,6 +184,29 @@ class KVPool:
         check(lib.rmlx_kv_decode_attention(self._h, layer, _ptr(q), q_heads_per_kv, _ptr(block_tables),
                                            block_table_stride, _ptr(seq_lens), num_seqs, softmax_scale, _ptr(out),
                                            _ptr(workspace), workspace_bytes, _stream(stream, self.device)))
+
+    def chunk_attention_workspace_size(self, q_heads_per_kv: int) -> int:
+        n = C.c_size_t()
+        check(lib.rmlx_kv_chunk_attention_workspace_size(self._h, q_heads_per_kv, C.byref(n)))
+        return n.value
+
+    def chunk_attention(self, layer: int, q, q_heads_per_kv: int, block_tables, block_table_stride: int, q_lens,
+                        seq_lens, num_seqs: int, num_q_tokens: int, softmax_scale: float, out, workspace,
+                        window: int = 0, q_token_stride: Optional[int] = None, q_head_stride: Optional[int] = None,
+                        workspace_bytes: Optional[int] = None, stream=None) -> None:
+        """Causal attention of each sequence's last q_lens[s] tokens over its
+        seq_lens[s] cached rows (the chunk's own included), `window` keys
+        back when it is not 0.  q strides are in elements and default to
+        contiguous [tokens][query heads][head_dim]."""
+        c = self.cfg
+        if workspace_bytes is None:
+            workspace_bytes = workspace.numel() * workspace.element_size()
+        qhs = c.head_dim if q_head_stride is None else q_head_stride
+        qts = c.num_kv_heads * q_heads_per_kv * c.head_dim if q_token_stride is None else q_token_stride
+        check(lib.rmlx_kv_chunk_attention(self._h, layer, _ptr(q), qts, qhs, q_heads_per_kv, _ptr(block_tables),
+                                          block_table_stride, _ptr(q_lens), _ptr(seq_lens), num_seqs, num_q_tokens,
+                                          softmax_scale, window, _ptr(out), _ptr(workspace), workspace_bytes,
+                                          _stream(stream, self.device)))
 
     def gather_ring(self, layer: int, block_tables, block_table_stride: int, seq_lens, ring_offsets, num_seqs: int,
                     keep: int, max_size: int, out_k, out_v, stream=None) -> None:
