@@ -19,6 +19,7 @@ enum : int32_t {
   DEV_ERR_WORKSPACE = 4,  // a launch's splits exceed the workspace it was given
   DEV_ERR_AXIS = 8,       // pair_axis entry outside [0, num_axes)
   DEV_ERR_Q_ROWS = 16,    // q_lens sum past the num_q_tokens rows of a launch
+  DEV_ERR_TIMEOUT = 32,   // a bounded wait inside a kernel ran out
 };
 
 // 16-byte streaming load through the non-coherent path without L1

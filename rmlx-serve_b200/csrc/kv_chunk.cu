@@ -8,10 +8,14 @@
 // h * G + g, with KV head h:
 //   out = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m).
 // A token that sees no key gives zeros.
+#include <cuda.h>
+
 #include <algorithm>
+#include <numeric>
 
 #include "dequant.cuh"
 #include "kv_pool_internal.cuh"
+#include "tcgen05.cuh"
 
 namespace rmlx {
 
@@ -21,6 +25,7 @@ struct ChunkArgs {
   const int32_t *bt, *q_lens, *seq_lens;
   int64_t qts, qhs;  // byte strides of q: token, head
   int layer, G, bt_stride, nseq, nq, window;
+  int max_len;  // rows that a row of the block tables can hold
   int gs_log2, bits, mf32;
   float scale_log2;
 };
@@ -99,44 +104,820 @@ __device__ __forceinline__ void attend_row(const PoolGeo& g, const ChunkArgs& a,
   }
 }
 
-// One warp per (token, query head).
-template <int DT, int HD>
-__global__ void __launch_bounds__(256) chunk_attn_rows_kernel(PoolGeo g, ChunkArgs a, int32_t* err) {
-  constexpr int EPL = HD / 32;
-  extern __shared__ int32_t smem[];
-  int32_t* cub = smem;
-  int32_t* cut = smem + a.nseq + 1;
+// ---------------------------------------------------------------------------
+// The plan.  A tile is up to 256 query rows of one sequence and KV head: the
+// G query heads of 256 / G consecutive chunk tokens, so that every K/V row
+// loaded serves all of them.  An item is (tile, KV head) with the 128-key
+// tiles that its mask leaves; its cost is that number plus CH_OVERHEAD.  The
+// launch's items are laid end to end and cut into equal shares, one per CTA,
+// so a share may begin and end inside an item: such portions write partial
+// results that a second kernel joins.  Every CTA works out its own share from
+// q_lens and seq_lens, with no counter shared between CTAs or launches.
+// ---------------------------------------------------------------------------
+constexpr int CH_ROWS = 256;    // query rows of a tile: two M = 128 accumulators
+constexpr int CH_KEYS = 128;    // keys of a key tile
+constexpr int CH_THREADS = 384; // two softmax warpgroups, one warpgroup of MMA and load warps
+constexpr int CH_OVERHEAD = 1;  // cost of an item besides its key tiles, in key tiles
+constexpr int CH_MIN_COST = 4;  // smallest share
+
+// Chunk token range, key tiles and masks of tile mt of a sequence.
+struct TileGeo {
+  int t0, rows, pos0, k_lo, nk, hi;  // first token, rows, its position, first key tile, key tiles, keys end (exclusive)
+};
+__device__ __forceinline__ TileGeo tile_geo(int qlen, int len, int mt, int tpt, int G, int window) {
+  TileGeo t;
+  t.t0 = mt * tpt;
+  const int n = min(tpt, qlen - t.t0);
+  t.rows = n * G;
+  t.pos0 = len - qlen + t.t0;
+  t.hi = t.pos0 + n;
+  const int lo = window && t.pos0 >= window ? t.pos0 - window + 1 : 0;
+  t.k_lo = lo / CH_KEYS;
+  t.nk = t.hi > 0 ? (t.hi - 1) / CH_KEYS + 1 - t.k_lo : 0;
+  return t;
+}
+
+// A CTA's place in the plan, walked item by item by every warp.
+struct ItemIter {
+  int s, mt, head, qoff, qlen, len;
+  int64_t off, left;  // position inside the item's cost, cost left in the share
+  // the current portion
+  TileGeo t;
+  int k0, k1;   // its key tiles, relative to t.k_lo
+  bool starts;  // it holds the item's beginning
+};
+__device__ __forceinline__ bool next_portion(ItemIter& it, const ChunkArgs& a, int heads, int tpt, bool first) {
+  if (!first) {
+    it.off = 0;
+    if (++it.head == heads) {
+      it.head = 0;
+      if ((++it.mt) * tpt >= it.qlen) it.mt = 0, it.qoff += it.qlen, it.qlen = 0;
+    }
+  }
+  if (it.left <= 0) return false;
+  while (it.qlen <= 0) {  // the next sequence with chunk tokens
+    if (++it.s >= a.nseq) return false;
+    it.qlen = max(__ldg(a.q_lens + it.s), 0);
+    it.len = min(max(__ldg(a.seq_lens + it.s), 0), a.max_len);
+  }
+  it.t = tile_geo(it.qlen, it.len, it.mt, tpt, a.G, a.window);
+  const int64_t end = min(it.off + it.left, (int64_t)it.t.nk + CH_OVERHEAD);
+  it.left -= end - it.off;
+  it.starts = it.off == 0;
+  it.k0 = (int)max(it.off - CH_OVERHEAD, (int64_t)0);
+  it.k1 = (int)max(end - CH_OVERHEAD, (int64_t)0);
+  return true;
+}
+
+// Sum of x over the CTA's earlier threads; *total over all.  words: 12 64-bit words of shared memory.
+__device__ __forceinline__ int64_t block_prefix(int64_t x, int64_t* words, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t y = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
+  }
+  __syncthreads();
+  if (lane == 31) words[warp] = y;
+  __syncthreads();
+  int64_t before = y - x, all = 0;
+#pragma unroll
+  for (int w = 0; w < CH_THREADS / 32; ++w) {
+    if (w < warp) before += words[w];
+    all += words[w];
+  }
+  *total = all;
+  return before;
+}
+
+// Cuts the work and leaves this CTA's share in *out (left = 0: none).
+// scratch: 2 (nseq + 1) words, 12 64-bit words.  False when q_lens sum past
+// a.nq.  Each thread walks a run of sequences, then a run of tiles.
+__device__ __forceinline__ bool make_plan(const ChunkArgs& a, int heads, int tpt, uint8_t* scratch, ItemIter* out,
+                                          int32_t* err) {
+  int64_t* words = reinterpret_cast<int64_t*>(scratch);
+  int32_t* cub = reinterpret_cast<int32_t*>(words + CH_THREADS / 32);  // tiles before a sequence
+  int32_t* cut = cub + a.nseq + 1;                                     // chunk tokens before it
+  const int tid = threadIdx.x;
+  if (tid == 0) out->left = 0;
+  const int per_s = (a.nseq + CH_THREADS - 1) / CH_THREADS;
+  const int s0 = min(a.nseq, tid * per_s), s1 = min(a.nseq, s0 + per_s);
+  int64_t tokens = 0, tiles = 0, total;
+  for (int s = s0; s < s1; ++s) {
+    const int q = max(__ldg(a.q_lens + s), 0);
+    tokens += q;
+    tiles += ((int64_t)q + tpt - 1) / tpt;
+    if (q > 0 && __ldg(a.seq_lens + s) > a.max_len && blockIdx.x == 0) atomicOr(err, DEV_ERR_BLOCK);
+  }
+  int64_t before = block_prefix(tokens, words, &total);
+  if (total > a.nq) return false;
+  int64_t tile = block_prefix(tiles, words, &total);
+  for (int s = s0; s < s1; ++s) {
+    cub[s] = (int32_t)tile, cut[s] = (int32_t)before;
+    const int q = max(__ldg(a.q_lens + s), 0);
+    before += q;
+    tile += (q + tpt - 1) / tpt;
+  }
+  if (s0 < s1 && s1 == a.nseq) cub[a.nseq] = (int32_t)tile, cut[a.nseq] = (int32_t)before;
+  __syncthreads();
+  const int T = cub[a.nseq], per = (T + CH_THREADS - 1) / CH_THREADS;
+  const int beg = (int)min((int64_t)T, (int64_t)tid * per), end = min(T, beg + per);
+  auto walk = [&](auto&& f) {  // f(sequence, its chunk length, its rows, tile, tile's cost over all heads)
+    if (beg >= end) return;
+    int s = find_seq(cub, a.nseq, beg);
+    for (int i = beg; i < end; ++s) {
+      const int qlen = cut[s + 1] - cut[s], len = min(max(__ldg(a.seq_lens + s), 0), a.max_len);
+      for (const int stop = min(end, cub[s + 1]); i < stop; ++i) {
+        const int mt = i - cub[s];
+        f(s, qlen, len, mt, (int64_t)heads * (tile_geo(qlen, len, mt, tpt, a.G, a.window).nk + CH_OVERHEAD));
+      }
+    }
+  };
+  int64_t mine = 0;
+  walk([&](int, int, int, int, int64_t c) { mine += c; });
+  before = block_prefix(mine, words, &total);
+  const int64_t n = max((int64_t)1, min((int64_t)gridDim.x, total / CH_MIN_COST));
+  if (blockIdx.x >= n) return true;
+  const int64_t b0 = total * blockIdx.x / n, b1 = total * (blockIdx.x + 1) / n;
+  if (b0 < b1 && before <= b0 && b0 < before + mine) {
+    int64_t c0 = before;
+    walk([&](int s, int qlen, int len, int mt, int64_t c) {
+      if (c0 <= b0 && b0 < c0 + c) {
+        const int64_t one = c / heads;
+        out->s = s, out->mt = mt, out->qoff = cut[s], out->qlen = qlen, out->len = len;
+        out->head = (int)((b0 - c0) / one), out->off = (b0 - c0) % one;
+        out->left = b1 - b0;
+      }
+      c0 += c;
+    });
+  }
+  return true;
+}
+
+// One partial result in the workspace: CH_ROWS unnormalised output rows, then
+// a (max, sum) pair per row; what it is a part of in a descriptor.  Slot 0 of
+// a CTA continues an item that an earlier CTA began, slot 1 begins one that a
+// later CTA goes on with.
+struct PartDesc {
+  int32_t valid, last, token0, head, rows, pad[3];
+};
+__host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROWS * (hd + 2); }
+
+// ---------------------------------------------------------------------------
+// The kernel.  S = Q K^T and O += P V on the tcgen05 tensor cores, S, P and O
+// in TMEM, K and V in a ring of shared-memory stages.  Warps 0-3 and 4-7 are
+// two softmax warpgroups (A and B) with an S/P and an O accumulator each, one
+// thread a row; warp 8 issues the MMAs; warp 9 loads K and V tiles by TMA and
+// warps 10-11 the queries (pools that TMA cannot read: warps 9-11 load all).
+//   more than 128 rows: A and B hold rows 0-127 and 128-255 and every key tile
+//     is used twice;
+//   up to 128 rows: A and B hold the same rows and take the even and the odd
+//     key tiles, joined at the end.
+// While one warpgroup does its softmax the tensor cores work for the other.
+// P overwrites the first half of its S.  O is rescaled only when a row's
+// maximum has grown by more than 2^8 since the last time (weights stay below
+// 2^8, exact in the accumulation's f32); the final division undoes it.
+//
+// A V row that the mask hides is weighed with 0, which leaves NaN where it
+// holds infinities or NaN.  Rows behind the last visible key are zeroed in
+// shared memory; should a row's output come out NaN all the same, its warp
+// computes that row again from the pool, reading visible rows only.
+//
+// Quantised pools: codes are dequantised to f16 in shared memory and the
+// products run in f16 (11 bits; bf16's 8 would add more error than the codes),
+// a bf16 query row scaled by a power of two into f16's range.  Groups whose
+// values leave f16's range become NaN, and their rows take the slow path.
+// ---------------------------------------------------------------------------
+struct ChunkParams {
+  PoolGeo g;
+  ChunkArgs a;
+  int tpt;                 // chunk tokens of a tile
+  int box;                 // rows of a TMA box
+  float* parts;
+  PartDesc* desc;
+};
+
+template <int HD>
+struct ChunkSmem {
+  static constexpr int HALVES = HD / 64;
+  static constexpr int QTILE = 128 * HD * 2;
+  static constexpr int STAGE = CH_KEYS * HD * 2;
+  static constexpr int STAGES = HD == 128 ? 5 : 8;
+  static constexpr int Q = 0, KV = 2 * QTILE, CTRL = KV + STAGES * STAGE;
+  // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales
+  static constexpr int BARS = CTRL, PLAN = CTRL + 256, ML = PLAN + 128, QSCALE = ML + 1024;
+  static constexpr int BYTES = QSCALE + 512;
+};
+// barrier numbers
+constexpr int BAR_FULL = 0, BAR_EMPTY = 8, BAR_QFULL = 16, BAR_QEMPTY = 17, BAR_S = 18, BAR_P = 20, BAR_O = 22,
+              BAR_OFREE = 24, BAR_ML = 25, BAR_DRAIN = 26;
+
+template <int DT>
+__device__ __forceinline__ float unpack_lo(uint32_t w) {
+  return DT == RMLX_BF16 ? __uint_as_float(w << 16) : __half2float(__ushort_as_half((uint16_t)w));
+}
+template <int DT>
+__device__ __forceinline__ float unpack_hi(uint32_t w) {
+  return DT == RMLX_BF16 ? __uint_as_float(w & 0xffff0000u) : __half2float(__ushort_as_half((uint16_t)(w >> 16)));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (DT == RMLX_BF16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Byte offset of 16-byte column c of row r in an operand tile: 128-byte
+// swizzled atoms of 8 rows x 64 elements.  Query tiles keep a half's 128 rows
+// together; K/V stages keep the halves of each 8 rows together, as a TMA box
+// of a block's rows leaves them.
+template <int HD>
+__device__ __forceinline__ uint32_t q_off(int r, int c) {
+  return (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+template <int HD>
+__device__ __forceinline__ uint32_t kv_off(int r, int c) {
+  return (r >> 3) * (HD * 16) + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// Eight elements of a stored row as f16 pairs.  w: 8-bit codes in both words,
+// 4-bit codes in w.x.  The group's values lie between zr and zr + qmax sc.
+template <int BITS>
+__device__ __forceinline__ uint4 dequant8(uint2 w, float sc, float zr, bool mf32, bool is_v) {
+  const float ma = fmaxf(fabsf(zr), fabsf(fmaf((float)((1 << BITS) - 1), sc, zr)));
+  if (!(ma <= 65504.0f) || (is_v && ma > 0.0f && ma < 3.0517578125e-5f)) sc = __uint_as_float(0x7fffffffu);
+  uint4 r;
+  uint32_t* o = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t m;  // two codes as f16 1024 + code
+    if (BITS == 8) {
+      m = __byte_perm(i < 2 ? w.x : w.y, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
+    } else {
+      const uint32_t b = w.x >> (8 * i);
+      m = 0x64006400u | (b & 15) | ((b & 0xf0) << 12);
+    }
+    const __half2 c = __hsub2(*reinterpret_cast<__half2*>(&m), __floats2half2_rn(1024.0f, 1024.0f));
+    __half2 v;
+    if (mf32) {
+      const float2 f = __half22float2(c);
+      v = __floats2half2_rn(fmaf(f.x, sc, zr), fmaf(f.y, sc, zr));
+    } else {  // f16 scale and zero: one rounding
+      v = __hfma2(c, __float2half2_rn(sc), __float2half2_rn(zr));
+    }
+    o[i] = *reinterpret_cast<uint32_t*>(&v);
+  }
+  return r;
+}
+
+template <int DT, int HD, int BITS, bool TMA>
+__global__ void __launch_bounds__(CH_THREADS, 1)
+    chunk_attn_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map, int32_t* err) {
+  using S = ChunkSmem<HD>;
+  constexpr int CT = BITS ? RMLX_F16 : DT;  // type of the products' operands
+  constexpr int ST = S::STAGES;
+  constexpr uint32_t IDESC_S = mma_idesc(CT == RMLX_BF16, 128, CH_KEYS, false);
+  constexpr uint32_t IDESC_O = mma_idesc(CT == RMLX_BF16, 128, HD, true);
+  constexpr uint32_t TM_S = 0, TM_O = 256;  // TMEM columns: S/P of A and B, then O of A and B
+  constexpr int QWARPS = TMA ? 2 : 3;       // warps that load queries
+  extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms are 1024 bytes
+  const uint32_t sb = smem_u32(smem);
+  const PoolGeo& g = p.g;
+  const ChunkArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto bar = [&](int i) { return sb + S::BARS + 8 * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + 240);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 244);
+  ItemIter* plan = reinterpret_cast<ItemIter*>(smem + S::PLAN);
+  float2* ml_b = reinterpret_cast<float2*>(smem + S::ML);
+  uint8_t* qscale = smem + S::QSCALE;  // [2][CH_ROWS] f32 exponents, by item parity
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(bar(BAR_FULL + i), TMA ? 1 : 3);
+      mbar_init(bar(BAR_EMPTY + i), 1);
+    }
+    mbar_init(bar(BAR_QFULL), QWARPS);
+    mbar_init(bar(BAR_QEMPTY), 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(bar(BAR_S + x), 1);
+      mbar_init(bar(BAR_P + x), 4);
+      mbar_init(bar(BAR_O + x), 1);
+    }
+    mbar_init(bar(BAR_OFREE), 8);
+    mbar_init(bar(BAR_ML), 4);
+    mbar_init(bar(BAR_DRAIN), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tmem_alloc(sb + S::BARS + 244, 512);
   pdl_wait();
   pdl_release();
-  scan_seq_lens(a.q_lens, a.nseq, 1, cub, cut);
-  if (cut[a.nseq] > a.nq) {
-    if (threadIdx.x == 0) atomicOr(err, DEV_ERR_Q_ROWS);
-    return;
+  PartDesc* desc = p.desc + 2 * blockIdx.x;
+  if (threadIdx.x < 2) desc[threadIdx.x].valid = 0;
+  if (!make_plan(a, g.heads, p.tpt, smem + S::KV, plan, err) && threadIdx.x == 0) atomicOr(err, DEV_ERR_Q_ROWS);
+  fence_async_smem();  // the plan's scratch becomes the K/V ring
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ItemIter it = *plan;
+  const int qheads = g.heads * a.G;
+
+  if (warp < 8) {
+    // ---- softmax warpgroups -----------------------------------------------
+    const int x = warp >> 2, wq = warp & 3;
+    const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
+    const uint32_t tm_s = tmem + lane_off + TM_S + 128 * x, tm_o = tmem + lane_off + TM_O + HD * x;
+    uint32_t ns = 0, nitem = 0, nml = 0, no[2] = {0, 0};  // phases: S tiles, items, (max, sum) handed over, O of A and B
+    for (bool more = next_portion(it, a, g.heads, p.tpt, true); more;
+         more = next_portion(it, a, g.heads, p.tpt, false)) {
+      const int nk = it.k1 - it.k0;
+      const bool two = it.t.rows > 128;
+      const int row = (two ? 128 * x : 0) + wq * 32 + lane;
+      const int tok = row / a.G, gq = row - tok * a.G;
+      const bool valid = row < it.t.rows;
+      const int64_t orow = (int64_t)(it.qoff + it.t.t0 + tok) * qheads + it.head * a.G + gq;
+      if (nk == 0) {
+        // an item with no visible key at all: zeros
+        if (it.starts && it.t.nk == 0 && valid && (two || x == 0)) {
+          uint4* o = reinterpret_cast<uint4*>(p.a.out + orow * HD * 2);
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) o[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        continue;
+      }
+      const int mine = two ? nk : (x == 0 ? (nk + 1) / 2 : nk / 2);
+      const bool active = (two ? 128 * x : 0) + wq * 32 < it.t.rows;
+      const int pos = it.t.pos0 + tok;
+      const int lim = valid ? max(pos + 1, 0) : INT32_MAX;  // visible keys: low <= key < lim
+      const int low = valid && a.window && pos >= a.window ? pos - a.window + 1 : 0;
+      float m = -INFINITY, l = 0.0f, c = a.scale_log2;
+      bool ok = true;
+      for (int j = 0; j < mine; ++j) {
+        if (!(ok = mbar_wait(bar(BAR_S + x), ns & 1, abort_flag, err))) break;
+        ++ns;
+        if (active) {
+          tc_fence_after();
+          if (BITS && j == 0) c = a.scale_log2 * __uint_as_float((uint32_t)qscale[(nitem & 1) * CH_ROWS + row] << 23);
+          uint32_t v[128];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, v + 32 * i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld_wait32(v + 32 * i);
+          const int kb = (it.t.k_lo + it.k0 + (two ? j : 2 * j + x)) * CH_KEYS;
+          if (__any_sync(0xffffffffu, kb + CH_KEYS > lim || kb < low)) {
+            const int r1 = lim - kb, r0 = low - kb;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i >= r1 || i < r0) v[i] = 0xff800000u;  // -inf
+          }
+          float mx = __uint_as_float(v[0]);
+#pragma unroll
+          for (int i = 1; i < 128; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+          if (__any_sync(0xffffffffu, (mx - m) * c > 8.0f)) {
+            const float n = fmaxf(m, mx);
+            const float f = n == m ? 1.0f : ex2((m - n) * c);
+            m = n;
+            l *= f;
+            if (j > 0) {
+#pragma unroll 1
+              for (int i = 0; i < HD; i += 32) {
+                uint32_t o[32];
+                tmem_ld32(tm_o + i, o);
+                tmem_ld_wait32(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st32(tm_o + i, o);
+              }
+              tc_wait_st();
+            }
+          }
+          const float nb = m == -INFINITY ? 0.0f : -m * c;
+          float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float e0 = ex2(fmaf(__uint_as_float(v[64 * h + 2 * i]), c, nb));
+              const float e1 = ex2(fmaf(__uint_as_float(v[64 * h + 2 * i + 1]), c, nb));
+              sum0 += e0;
+              sum1 += e1;
+              w[i] = pack2<CT>(e0, e1);
+            }
+            tmem_st32(tm_s + 32 * h, w);
+          }
+          l += sum0 + sum1;
+          tc_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(BAR_P + x));
+      }
+      if (!ok) break;
+      // ---- epilogue ---------------------------------------------------------
+      float ml = m == -INFINITY ? -INFINITY : m * c;  // in the log2 domain
+      const bool whole = it.k0 == 0 && it.k1 == it.t.nk;
+      const int slot = it.k0 == 0 ? 1 : 0;
+      float* part = p.parts + (size_t)(2 * blockIdx.x + slot) * part_floats(HD);
+      if (!whole && threadIdx.x == 0) {
+        desc[slot].last = it.k1 == it.t.nk, desc[slot].token0 = it.qoff + it.t.t0;
+        desc[slot].head = it.head, desc[slot].rows = it.t.rows, desc[slot].valid = 1;
+      }
+      bool writes = active;
+      float fa = 1.0f, fb = 0.0f;
+      const bool has[2] = {true, two || nk > 1};  // A and B have tiles
+      if (!two) {
+        if (x == 1) {
+          if (nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, abort_flag, err))) break;
+          ml_b[wq * 32 + lane] = make_float2(ml, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(BAR_ML));
+          writes = false;
+        } else {
+          if (!(ok = mbar_wait(bar(BAR_ML), nml & 1, abort_flag, err))) break;
+          const float2 b = ml_b[wq * 32 + lane];
+          const float n = fmaxf(ml, b.x);
+          const float base = n == -INFINITY ? 0.0f : n;
+          fa = ex2(ml - base);
+          fb = ex2(b.x - base);  // 0 without tiles
+          l = l * fa + b.y * fb;
+          ml = n;
+        }
+        ++nml;
+      }
+#pragma unroll
+      for (int y = 0; y < 2 && ok; ++y) {
+        // a warpgroup reads its own O, and A reads B's too when they share rows
+        if (has[y] && (y == x || (!two && x == 0))) ok = mbar_wait(bar(BAR_O + y), no[y] & 1, abort_flag, err);
+        no[y] += has[y];
+      }
+      if (!ok) break;
+      ++nitem;
+      if (writes) {
+        tc_fence_after();
+        const float il = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        float nan = l;  // becomes NaN with any NaN among the outputs
+#pragma unroll 1
+        for (int i = 0; i < HD; i += 32) {
+          uint32_t o[32];
+          tmem_ld32(tm_o + i, o);
+          tmem_ld_wait32(o);
+          float f[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]);
+          if (!two) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] *= fa;
+            if (has[1]) {
+              tmem_ld32(tm_o + HD + i, o);
+              tmem_ld_wait32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = fmaf(__uint_as_float(o[e]), fb, f[e]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            f[e] = l == 0.0f ? 0.0f : f[e] * il;
+            nan = fmaf(f[e], 0.0f, nan);
+          }
+          if (valid) {
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(p.a.out + (orow * HD + i) * 2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                dst[e] = make_uint4(pack2<DT>(f[8 * e], f[8 * e + 1]), pack2<DT>(f[8 * e + 2], f[8 * e + 3]),
+                                    pack2<DT>(f[8 * e + 4], f[8 * e + 5]), pack2<DT>(f[8 * e + 6], f[8 * e + 7]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(part + (size_t)row * HD + i);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+            }
+          }
+        }
+        if (valid && !whole) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[row] = make_float2(ml, l);
+        // rows whose output holds NaN: again, from visible rows only
+        unsigned bad = __ballot_sync(0xffffffffu, valid && nan != nan);
+        while (bad) {
+          const int b = __ffs(bad) - 1;
+          bad &= bad - 1;
+          const int br = __shfl_sync(0xffffffffu, row, b), blim = __shfl_sync(0xffffffffu, lim, b),
+                    blow = __shfl_sync(0xffffffffu, low, b);
+          const int64_t bo = __shfl_sync(0xffffffffu, orow, b);
+          const int bt = br / a.G, bg = br - bt * a.G;
+          constexpr int EPL = HD / 32;
+          float qf[EPL], acc[EPL], bm = -INFINITY, bl = 0.0f;
+          const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q + (it.qoff + it.t.t0 + bt) * a.qts +
+                                                                 (it.head * a.G + bg) * a.qhs) + lane * EPL;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) qf[e] = unpack_lo<DT>(__ldg(qp + e)), acc[e] = 0.0f;
+          const int k_first = (it.t.k_lo + it.k0) * CH_KEYS, k_end = (it.t.k_lo + it.k1) * CH_KEYS;
+          attend_row<DT, HD>(g, a, a.bt + (int64_t)it.s * a.bt_stride, it.head, max(blow, k_first), min(blim, k_end),
+                             qf, lane, err, bm, bl, acc);
+          const float bi = whole ? (bl == 0.0f ? 0.0f : 1.0f / bl) : 1.0f;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            const float y = acc[e] * bi;
+            if (whole)
+              reinterpret_cast<uint16_t*>(p.a.out)[bo * HD + lane * EPL + e] = (uint16_t)pack2<DT>(y, 0.0f);
+            else
+              part[(size_t)br * HD + lane * EPL + e] = y;
+          }
+          if (!whole && lane == 0) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[br] = make_float2(bm, bl);
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(BAR_OFREE));
+    }
+  } else if (warp == 8) {
+    // ---- MMA issue ----------------------------------------------------------
+    uint32_t n = 0, nitem = 0, np[2] = {0, 0};
+    bool ok = true;
+    const uint32_t q_base = sb + S::Q, kv_base = sb + S::KV;
+    auto full = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_FULL + i % ST), (i / ST) & 1, abort_flag, err); };
+    auto scores = [&](int x, int qt, uint32_t stage) {  // S_x = Q_qt K^T
+      if (lane == 0) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint64_t qd = smem_desc(q_base + qt * S::QTILE + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024);
+          const uint64_t kd = smem_desc(kv_base + stage * S::STAGE + (kk >> 2) * 1024 + (kk & 3) * 32, 16, HD * 16);
+          mma_ss(tmem + TM_S + 128 * x, qd, kd, IDESC_S, kk > 0);
+        }
+        tc_commit(bar(BAR_S + x));
+      }
+    };
+    auto values = [&](int x, uint32_t stage, int steps, bool first) {  // O_x (+)= P_x V
+      if (lane == 0) {
+        for (int kk = 0; kk < steps; ++kk)
+          mma_ts(tmem + TM_O + HD * x, tmem + TM_S + 128 * x + 8 * kk,
+                 smem_desc(kv_base + stage * S::STAGE + kk * (HD * 32), 1024, HD * 16), IDESC_O, !(first && kk == 0));
+      }
+    };
+    for (bool more = next_portion(it, a, g.heads, p.tpt, true); more;
+         more = next_portion(it, a, g.heads, p.tpt, false)) {
+      const int nk = it.k1 - it.k0;
+      if (nk == 0) continue;
+      const bool two = it.t.rows > 128;
+      const int lead = two ? 1 : min(2, nk);
+      if (!(ok = mbar_wait(bar(BAR_QFULL), nitem & 1, abort_flag, err))) break;
+      for (int i = 0; i < lead && ok; ++i) {
+        if (!full(n)) break;
+        tc_fence_after();
+        scores(two ? 0 : i, 0, n % ST);
+        if (two) scores(1, 1, n % ST);
+        if (lane == 0) tc_commit(bar(BAR_EMPTY + n % ST));
+        ++n;
+      }
+      if (!ok) break;
+      if (lead == nk && lane == 0) tc_commit(bar(BAR_QEMPTY));
+      for (int j = 0; j < nk; ++j) {
+        const uint32_t sv = n++;  // V of tile j; then K of tile j + lead
+        const bool k_next = j + lead < nk;
+        const uint32_t sk = n;
+        if (k_next) ++n;
+        if (!full(sv)) break;
+        const int keys = min(CH_KEYS, it.t.hi - (it.t.k_lo + it.k0 + j) * CH_KEYS);
+        const int steps = (keys + 15) / 16;
+        if (TMA && (keys & 15)) {
+          // keys behind the last visible one that share its MMA step: zeros
+          for (int i = lane; i < (16 * steps - keys) * (HD / 8); i += 32)
+            sts128(kv_base + (sv % ST) * S::STAGE + kv_off<HD>(keys + i / (HD / 8), i % (HD / 8)), make_uint4(0u, 0u, 0u, 0u));
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (j == 0 && nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, abort_flag, err))) break;
+        for (int y = 0; y < (two ? 2 : 1); ++y) {
+          const int x = two ? y : j & 1;
+          if (!(ok = mbar_wait(bar(BAR_P + x), np[x] & 1, abort_flag, err))) break;
+          ++np[x];
+          tc_fence_after();
+          values(x, sv % ST, steps, two ? j == 0 : j < 2);
+          if (two ? j == nk - 1 : j >= nk - 2)
+            if (lane == 0) tc_commit(bar(BAR_O + x));
+          if (y == (two ? 1 : 0) && lane == 0) tc_commit(bar(BAR_EMPTY + sv % ST));
+          if (k_next) {
+            if (y == 0) {
+              if (!full(sk)) break;
+              tc_fence_after();
+            }
+            scores(x, two ? y : 0, sk % ST);
+            if (y == (two ? 1 : 0) && lane == 0) {
+              tc_commit(bar(BAR_EMPTY + sk % ST));
+              if (j + lead == nk - 1) tc_commit(bar(BAR_QEMPTY));
+            }
+          }
+        }
+        if (!ok) break;
+      }
+      if (!ok) break;
+      ++nitem;
+    }
+    if (!ok) {  // leave no MMA in flight behind
+      if (lane == 0) tc_commit(bar(BAR_DRAIN));
+      for (int i = 0; i < (1 << 20) && !mbar_try(bar(BAR_DRAIN), 0); ++i) {
+      }
+    }
+  } else {
+    // ---- loads ----------------------------------------------------------------
+    uint32_t n = 0, nitem = 0;
+    bool ok = true;
+    const bool loads_q = !TMA || warp >= 10, loads_kv = !TMA || warp == 9;
+    const int qw = TMA ? warp - 10 : warp - 9;
+    const int64_t vdelta = (int64_t)g.heads * g.tile_bytes;
+    for (bool more = next_portion(it, a, g.heads, p.tpt, true); more;
+         more = next_portion(it, a, g.heads, p.tpt, false)) {
+      const int nk = it.k1 - it.k0;
+      if (nk == 0) continue;
+      const bool two = it.t.rows > 128;
+      const int32_t* btrow = a.bt + (int64_t)it.s * a.bt_stride;
+      if (loads_q) {
+        if (nitem > 0 && !(ok = mbar_wait(bar(BAR_QEMPTY), (nitem - 1) & 1, abort_flag, err))) break;
+        constexpr int CPR = HD / 8, RPW = 32 / CPR;  // 16-byte chunks of a row, rows of a warp's pass
+        const uint8_t* qbase = a.q + (int64_t)(it.qoff + it.t.t0) * a.qts + (int64_t)it.head * a.G * a.qhs;
+        const int ch = lane % CPR;
+        constexpr int U = 4;
+        for (int r0 = (qw * RPW) + lane / CPR; r0 < it.t.rows + (int)(lane / CPR); r0 += U * QWARPS * RPW) {
+          uint4 w[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * QWARPS * RPW;
+            w[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < it.t.rows) {
+              const int tok = r / a.G;
+              w[u] = ld_stream(qbase + tok * a.qts + (r - tok * a.G) * a.qhs + ch * 16);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * QWARPS * RPW;
+            if (BITS) {
+              // the row's power of two, and a bf16 row in f16
+              int e = 127;
+              if (DT == RMLX_BF16) {
+                uint32_t* q4 = reinterpret_cast<uint32_t*>(&w[u]);
+                float mx = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  mx = fmaxf(mx, fmaxf(fabsf(unpack_lo<DT>(q4[i])), fabsf(unpack_hi<DT>(q4[i]))));
+#pragma unroll
+                for (int o = 1; o < CPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                e = (int)(__float_as_uint(mx) >> 23);  // 2^(e - 127) <= max
+                if (e == 0 || e == 255) e = 127;       // zeros, infinities
+                const float inv = 1.0f / __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q4[i] = pack2<RMLX_F16>(unpack_lo<DT>(q4[i]) * inv, unpack_hi<DT>(q4[i]) * inv);
+              }
+              if (ch == 0 && r < CH_ROWS) qscale[(nitem & 1) * CH_ROWS + r] = (uint8_t)e;
+            }
+            if (r < it.t.rows)
+              sts128(sb + S::Q + (r >> 7) * S::QTILE + q_off<HD>(r & 127, ch), w[u]);
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(BAR_QFULL));
+      }
+      ++nitem;
+      if (!loads_kv) continue;
+      auto load = [&](int j, int kv) {
+        const uint32_t stage = n % ST, dst = sb + S::KV + stage * S::STAGE;
+        if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) return;
+        ++n;
+        const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
+        if constexpr (TMA) {
+          // one box of p.box rows a lane
+          const int t = kb + lane * p.box;
+          const bool want = lane * p.box < CH_KEYS && t < it.t.hi;
+          int blk = 0, b = 0;
+          if (want) {
+            b = t / g.bs;
+            blk = b < a.bt_stride ? __ldg(btrow + b) : -1;
+            if (blk < 0 || blk >= g.nblocks) {
+              atomicOr(err, DEV_ERR_BLOCK);
+              blk = 0;
+            }
+          }
+          const int boxes = __popc(__ballot_sync(0xffffffffu, want));
+          if (lane == 0) mbar_arrive_expect_tx(bar(BAR_FULL + stage), boxes * p.box * HD * 2);
+          __syncwarp();
+          if (want)
+            tma_load_4d(dst + lane * p.box * (HD * 2), &map, 0, 0, 0,
+                        (int)((((int64_t)blk * g.layers + a.layer) * 2 + kv) * g.heads + it.head) * (g.bs / 8) +
+                            (t - b * g.bs) / 8,
+                        bar(BAR_FULL + stage));
+        } else {
+          // units of 8 elements (plain) or of one 16-byte run of codes
+          constexpr int UPR = BITS ? HD * BITS / 128 : HD / 8;
+          for (int u = (warp - 9) * 32 + lane; u < CH_KEYS * UPR; u += 96) {
+            const int r = u / UPR, ch = u % UPR, t = kb + r;
+            const uint8_t* tile = nullptr;
+            int slot = 0;
+            if (t < it.t.hi) {
+              const int b = t / g.bs;
+              const int32_t blk = b < a.bt_stride ? __ldg(btrow + b) : -1;
+              if (blk < 0 || blk >= g.nblocks) atomicOr(err, DEV_ERR_BLOCK);
+              else tile = g.base + g.tile_off(blk, a.layer, 0, it.head) + kv * vdelta;
+              slot = t - b * g.bs;
+            }
+            if (!BITS) {
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if (tile) w = ld_stream(tile + (int64_t)slot * g.row_bytes + ch * 16);
+              sts128(dst + kv_off<HD>(r, ch), w);
+            } else {
+              constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8;  // elements of a unit
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if (tile) w = ld_stream(tile + (int64_t)slot * g.row_bytes + ch * 16);
+              const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
+              const uint8_t* meta = tile + (int64_t)g.bs * g.row_bytes + (int64_t)slot * g.meta_row_bytes;
+              float sc = 0.0f, zr = 0.0f;
+              int cur = -1;
+#pragma unroll
+              for (int i = 0; i < EPU / 8; ++i) {
+                const int q = (ch * EPU + 8 * i) >> a.gs_log2;
+                if (tile && q != cur) {
+                  cur = q;
+                  if (a.mf32) {
+                    const float2 m2 = __ldg(reinterpret_cast<const float2*>(meta) + q);
+                    sc = m2.x, zr = m2.y;
+                  } else {
+                    const uint32_t m2 = __ldg(reinterpret_cast<const uint32_t*>(meta) + q);
+                    sc = unpack_lo<RMLX_F16>(m2), zr = unpack_hi<RMLX_F16>(m2);
+                  }
+                }
+                const uint2 two8 = BITS == 8 ? make_uint2(cw[2 * (i & 1)], cw[2 * (i & 1) + 1]) : make_uint2(cw[i & 3], 0u);
+                sts128(dst + kv_off<HD>(r, ch * (EPU / 8) + i), dequant8<BITS ? BITS : 8>(two8, sc, zr, a.mf32, kv));
+              }
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(BAR_FULL + stage));
+        }
+      };
+      const int lead = two ? 1 : min(2, nk);
+      for (int i = 0; i < lead && ok; ++i) load(i, 0);
+      for (int j = 0; j < nk && ok; ++j) {
+        load(j, 1);
+        if (ok && j + lead < nk) load(j + lead, 0);
+      }
+      if (!ok) break;
+    }
+    if (TMA && !ok && loads_kv)  // leave no copy in flight behind
+      for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i)
+        for (int k = 0; k < (1 << 20) && !mbar_try(bar(BAR_FULL + i % ST), (i / ST) & 1); ++k) {
+        }
   }
-  const int lane = threadIdx.x & 31, qheads = g.heads * a.G;
-  const int64_t total = (int64_t)cut[a.nseq] * qheads;
-  const int64_t nwarps = ((int64_t)gridDim.x * blockDim.x) >> 5;
-  for (int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; w < total; w += nwarps) {
-    const int t = (int)(w / qheads), hq = (int)(w - (int64_t)t * qheads);
-    const int s = find_seq(cut, a.nseq, t);
-    const int n = cut[s + 1] - cut[s], len = max(__ldg(a.seq_lens + s), 0);
-    const int pos = len - n + (t - cut[s]);
-    float qf[EPL], acc[EPL], m = -INFINITY, l = 0.0f;
-    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q + t * a.qts + hq * a.qhs) + lane * EPL;
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_free(tmem, 512);
+}
+
+// Joins the portions of the items that more than one CTA worked on.  Block
+// (c, y): rows 32 y .. of the item that CTA c began and others went on with.
+template <int DT, int HD>
+__global__ void __launch_bounds__(256) chunk_combine_kernel(ChunkParams p, int nparts) {
+  constexpr int EPL = HD / 32;
+  pdl_release();
+  pdl_wait();
+  const PartDesc d = p.desc[2 * blockIdx.x + 1];
+  if (!d.valid || (int)blockIdx.y * 32 >= d.rows) return;
+  int end = blockIdx.x + 1;  // CTAs c + 1 .. end hold the rest
+  while (end < nparts - 1 && !p.desc[2 * end].last) ++end;
+  const int lane = threadIdx.x & 31;
+  for (int row = blockIdx.y * 32 + (threadIdx.x >> 5); row < min(d.rows, (int)blockIdx.y * 32 + 32); row += 8) {
+    float m = -INFINITY, l = 0.0f, acc[EPL];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      qf[e] = DT == RMLX_BF16 ? __uint_as_float((uint32_t)__ldg(qp + e) << 16) : __half2float(__ushort_as_half(__ldg(qp + e)));
-      acc[e] = 0.0f;
+    for (int e = 0; e < EPL; ++e) acc[e] = 0.0f;
+    for (int c = blockIdx.x; c <= end; ++c) {
+      const float* part = p.parts + (size_t)(2 * c + (c == (int)blockIdx.x)) * part_floats(HD);
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(part + (size_t)CH_ROWS * HD) + row);
+      const float n = fmaxf(m, x.x), base = n == -INFINITY ? 0.0f : n;
+      const float f0 = ex2(m - base), f1 = ex2(x.x - base);
+      m = n;
+      l = l * f0 + x.y * f1;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) acc[e] = acc[e] * f0 + __ldcg(part + (size_t)row * HD + lane * EPL + e) * f1;
     }
-    const int k0 = a.window && pos >= a.window ? pos - a.window + 1 : 0;
-    attend_row<DT, HD>(g, a, a.bt + (int64_t)s * a.bt_stride, hq / a.G, k0, pos + 1, qf, lane, err, m, l, acc);
     const float il = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + ((int64_t)t * qheads + hq) * HD + lane * EPL;
+    const int tok = row / p.a.G, gq = row - tok * p.a.G;
+    uint32_t* o = reinterpret_cast<uint32_t*>(
+        p.a.out + (((int64_t)(d.token0 + tok) * p.g.heads + d.head) * p.a.G + gq) * HD * 2 + lane * EPL * 2);
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      const float x = acc[e] * il;
-      o[e] = DT == RMLX_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
-    }
+    for (int e = 0; e < EPL; e += 2) o[e / 2] = pack2<DT>(acc[e] * il, acc[e + 1] * il);
   }
 }
 
@@ -144,12 +925,57 @@ __global__ void __launch_bounds__(256) chunk_attn_rows_kernel(PoolGeo g, ChunkAr
 
 using namespace rmlx;
 
+namespace {
+
+using ChunkFn = void (*)(ChunkParams, CUtensorMap, int32_t*);
+template <int DT, int HD>
+ChunkFn pick_chunk(int bits, bool tma) {
+  if (bits == 8) return chunk_attn_kernel<DT, HD, 8, false>;
+  if (bits == 4) return chunk_attn_kernel<DT, HD, 4, false>;
+  return tma ? chunk_attn_kernel<DT, HD, 0, true> : chunk_attn_kernel<DT, HD, 0, false>;
+}
+
+size_t chunk_workspace(const rmlx_kv_pool* p) {
+  return (size_t)p->num_sms * 2 * (part_floats(p->cfg.head_dim) * sizeof(float) + sizeof(PartDesc));
+}
+
+// The pool as TMA sees it: [group of 8 rows][64-column half][row][64 elements],
+// loaded a box of `box` rows at a time into 128-byte-swizzled shared memory.
+// Every coordinate but the group's is 0, so a box starts on a 16-byte boundary.
+rmlx_status chunk_map(rmlx_kv_pool* p, int box, CUtensorMap* map) {
+  using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeFn encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  if (!encode) return fail(RMLX_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const rmlx_pool_config& c = p->cfg;
+  const cuuint64_t hd = c.head_dim;
+  const cuuint64_t dims[4] = {64, 8, hd / 64, (cuuint64_t)c.num_blocks * c.num_layers * 2 * c.num_kv_heads * (c.block_size / 8)};
+  const cuuint64_t strides[3] = {hd * 2, 128, hd * 16};
+  const cuuint32_t boxes[4] = {64, 8, (cuuint32_t)hd / 64, (cuuint32_t)box / 8}, ones[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, c.dtype == RMLX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            4, p->base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(RMLX_E_CUDA, "cuTensorMapEncodeTiled: error %d", (int)r);
+  return RMLX_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 rmlx_status rmlx_kv_chunk_attention_workspace_size(const rmlx_kv_pool* p, int32_t q_heads_per_kv, size_t* bytes) {
   if (!p || !bytes) return fail(RMLX_E_BAD_ARG, "NULL pool or bytes");
   if (q_heads_per_kv < 1 || q_heads_per_kv > 16) return fail(RMLX_E_BAD_ARG, "q_heads_per_kv must be in [1, 16]");
-  *bytes = 16;
+  const int hd = p->cfg.head_dim;
+  *bytes = hd == 64 || hd == 128 ? chunk_workspace(p) : 0;
   return RMLX_OK;
 }
 
@@ -184,18 +1010,32 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   a.qts = qts, a.qhs = qhs;
   a.layer = layer, a.G = q_heads_per_kv, a.bt_stride = block_table_stride, a.nseq = num_seqs, a.nq = num_q_tokens;
   a.window = window;
+  a.max_len = (int)std::min<int64_t>((int64_t)block_table_stride * c.block_size, 1 << 30);
   a.gs_log2 = c.quant_bits ? log2i(c.group_size) : 0, a.bits = c.quant_bits, a.mf32 = c.meta_dtype == RMLX_F32;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;  // log2(e)
   DeviceGuard dg(p->device);
   const bool bf = c.dtype == RMLX_BF16;
-  auto fn = c.head_dim == 128 ? (bf ? chunk_attn_rows_kernel<RMLX_BF16, 128> : chunk_attn_rows_kernel<RMLX_F16, 128>)
-                              : (bf ? chunk_attn_rows_kernel<RMLX_BF16, 64> : chunk_attn_rows_kernel<RMLX_F16, 64>);
-  const size_t smem = (size_t)(num_seqs + 1) * 2 * sizeof(int32_t);
+  ChunkParams prm;
+  prm.g = p->geo();
+  prm.a = a;
+  prm.tpt = CH_ROWS / q_heads_per_kv;
+  // TMA reads whole groups of 8 stored rows; a box is the most rows that both a block and a key tile hold a whole number of
+  prm.box = std::gcd(c.block_size, CH_KEYS);
+  const bool tma = !c.quant_bits && c.block_size % 8 == 0;
+  prm.parts = static_cast<float*>(workspace);
+  prm.desc = reinterpret_cast<PartDesc*>(prm.parts + (size_t)p->num_sms * 2 * part_floats(c.head_dim));
+  CUtensorMap map = {};
+  if (tma && (s = chunk_map(p, prm.box, &map)) != RMLX_OK) return s;
+  ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
+                                 : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
+  const size_t smem = c.head_dim == 128 ? ChunkSmem<128>::BYTES : ChunkSmem<64>::BYTES;
   if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
-  const int64_t rows = (int64_t)num_q_tokens * c.num_kv_heads * q_heads_per_kv;
-  const int grid = (int)std::min<int64_t>((rows + 7) / 8, persistent_grid(fn, 256, smem, p->num_sms));
-  cudaError_t e = launch_pdl(fn, dim3(grid), dim3(256), smem, (cudaStream_t)stream, p->geo(), a, p->err);
+  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(CH_THREADS), smem, (cudaStream_t)stream, prm, map, p->err);
   if (e != cudaSuccess) return cuda_check(e, "chunk attention launch");
+  auto fc = c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
+                              : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>);
+  e = launch_pdl(fc, dim3(p->num_sms, CH_ROWS / 32), dim3(256), 0, (cudaStream_t)stream, prm, (int)p->num_sms);
+  if (e != cudaSuccess) return cuda_check(e, "chunk attention combine launch");
   return cuda_check(cudaGetLastError(), "chunk attention launch");
 }
 

@@ -412,6 +412,11 @@ def test_graphs_streams_and_bad_arguments(cuda):
     out.fill_(3.0)
     pool.chunk_attention(0, q, G, bt, bt.shape[1], dq, dl, 2, q.shape[0] - 1, D ** -0.5, out, ws)
     assert pool.check() == 16 and (out == 3.0).all()
+    pool.chunk_attention(0, q, G, bt, bt.shape[1], dev([2 ** 30] * 2), dl, 2, q.shape[0], D ** -0.5, out, ws)
+    assert pool.check() == 16 and (out == 3.0).all()
+    four = bt[[0, 1, 0, 1]].contiguous()  # lengths whose 32-bit sum is 0
+    pool.chunk_attention(0, q, G, four, bt.shape[1], dev([2 ** 30] * 4), dev([9] * 4), 4, q.shape[0], D ** -0.5, out, ws)
+    assert pool.check() == 16 and (out == 3.0).all()
     # a bad block of one sequence, a table that is too short for the other: flagged; a third is right
     bad = torch.cat([bt, bt[:1]])[:, :bt.shape[1]].contiguous()
     bad[0, 3] = 80
@@ -421,9 +426,10 @@ def test_graphs_streams_and_bad_arguments(cuda):
     pool.chunk_attention(0, q3, G, bad, bad.shape[1], dev(q_lens + [30]), dev(lens + [400]), 3, q3.shape[0], D ** -0.5, out3, ws)
     assert pool.check() == 2
     check(pool, 0, q3[35:], G, bad[2:].contiguous(), [30], [400], 0, out3[35:], dt)
-    pool.chunk_attention(0, q, G, bt, bt.shape[1], dq, dev([400, 10 ** 6]), 2, q.shape[0], D ** -0.5, out, ws)
-    assert pool.check() == 2
-    check(pool, 0, q[:30], G, bt[:1].contiguous(), [30], [400], 0, out[:30], dt)
+    for long in (10 ** 6, 2 ** 31 - 1):
+        pool.chunk_attention(0, q, G, bt, bt.shape[1], dq, dev([400, long]), 2, q.shape[0], D ** -0.5, out, ws)
+        assert pool.check() == 2
+        check(pool, 0, q[:30], G, bt[:1].contiguous(), [30], [400], 0, out[:30], dt)
 
     def refused(status=5, **kw):
         args = dict(layer=0, q=q, q_heads_per_kv=G, block_tables=bt, block_table_stride=bt.shape[1], q_lens=dq, seq_lens=dl,
