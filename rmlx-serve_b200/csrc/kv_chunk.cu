@@ -27,6 +27,7 @@ struct ChunkArgs {
   int layer, G, bt_stride, nseq, nq, window;
   int max_len;  // rows that a row of the block tables can hold
   int gs_log2, bits, mf32;
+  int bs_log2;  // of the block size, -1 when it is no power of two
   float scale_log2;
 };
 
@@ -79,7 +80,7 @@ __device__ __forceinline__ void attend_row(const PoolGeo& g, const ChunkArgs& a,
   const int64_t vdelta = (int64_t)g.heads * g.tile_bytes;
   for (int j = k0; j < k1; ++j) {
     const int b = j / g.bs;
-    const int32_t blk = b < a.bt_stride ? __ldg(btrow + b) : -1;
+    const int32_t blk = __ldg(btrow + b);
     if (blk < 0 || blk >= g.nblocks) {
       if (lane == 0) atomicOr(err, DEV_ERR_BLOCK);
       continue;
@@ -116,8 +117,12 @@ __device__ __forceinline__ void attend_row(const PoolGeo& g, const ChunkArgs& a,
 // ---------------------------------------------------------------------------
 constexpr int CH_ROWS = 256;    // query rows of a tile: two M = 128 accumulators
 constexpr int CH_KEYS = 128;    // keys of a key tile
-constexpr int CH_THREADS = 384; // two softmax warpgroups, one warpgroup of MMA and load warps
-constexpr int CH_OVERHEAD = 1;  // cost of an item besides its key tiles, in key tiles
+constexpr int CH_HALF = 64;     // keys whose weights are made together
+// Two softmax warpgroups, the MMA warp, and load warps: three with TMA, seven
+// where they read and dequantise rows themselves.
+constexpr int ch_threads(bool tma) { return tma ? 384 : 512; }
+constexpr int CH_MAX_WARPS = 16;
+constexpr int CH_OVERHEAD = 3;  // cost of an item besides its key tiles, in key tiles
 constexpr int CH_MIN_COST = 4;  // smallest share
 
 // Chunk token range, key tiles and masks of tile mt of a sequence.
@@ -169,7 +174,7 @@ __device__ __forceinline__ bool next_portion(ItemIter& it, const ChunkArgs& a, i
   return true;
 }
 
-// Sum of x over the CTA's earlier threads; *total over all.  words: 12 64-bit words of shared memory.
+// Sum of x over the CTA's earlier threads; *total over all.  words: CH_MAX_WARPS 64-bit words of shared memory.
 __device__ __forceinline__ int64_t block_prefix(int64_t x, int64_t* words, int64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t y = x;
@@ -182,8 +187,7 @@ __device__ __forceinline__ int64_t block_prefix(int64_t x, int64_t* words, int64
   if (lane == 31) words[warp] = y;
   __syncthreads();
   int64_t before = y - x, all = 0;
-#pragma unroll
-  for (int w = 0; w < CH_THREADS / 32; ++w) {
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
     if (w < warp) before += words[w];
     all += words[w];
   }
@@ -192,16 +196,16 @@ __device__ __forceinline__ int64_t block_prefix(int64_t x, int64_t* words, int64
 }
 
 // Cuts the work and leaves this CTA's share in *out (left = 0: none).
-// scratch: 2 (nseq + 1) words, 12 64-bit words.  False when q_lens sum past
+// scratch: CH_MAX_WARPS 64-bit words, 2 (nseq + 1) words.  False when q_lens sum past
 // a.nq.  Each thread walks a run of sequences, then a run of tiles.
 __device__ __forceinline__ bool make_plan(const ChunkArgs& a, int heads, int tpt, uint8_t* scratch, ItemIter* out,
                                           int32_t* err) {
   int64_t* words = reinterpret_cast<int64_t*>(scratch);
-  int32_t* cub = reinterpret_cast<int32_t*>(words + CH_THREADS / 32);  // tiles before a sequence
+  int32_t* cub = reinterpret_cast<int32_t*>(words + CH_MAX_WARPS);  // tiles before a sequence
   int32_t* cut = cub + a.nseq + 1;                                     // chunk tokens before it
   const int tid = threadIdx.x;
   if (tid == 0) out->left = 0;
-  const int per_s = (a.nseq + CH_THREADS - 1) / CH_THREADS;
+  const int nt = blockDim.x, per_s = (a.nseq + nt - 1) / nt;
   const int s0 = min(a.nseq, tid * per_s), s1 = min(a.nseq, s0 + per_s);
   int64_t tokens = 0, tiles = 0, total;
   for (int s = s0; s < s1; ++s) {
@@ -221,7 +225,7 @@ __device__ __forceinline__ bool make_plan(const ChunkArgs& a, int heads, int tpt
   }
   if (s0 < s1 && s1 == a.nseq) cub[a.nseq] = (int32_t)tile, cut[a.nseq] = (int32_t)before;
   __syncthreads();
-  const int T = cub[a.nseq], per = (T + CH_THREADS - 1) / CH_THREADS;
+  const int T = cub[a.nseq], per = (T + nt - 1) / nt;
   const int beg = (int)min((int64_t)T, (int64_t)tid * per), end = min(T, beg + per);
   auto walk = [&](auto&& f) {  // f(sequence, its chunk length, its rows, tile, tile's cost over all heads)
     if (beg >= end) return;
@@ -255,8 +259,8 @@ __device__ __forceinline__ bool make_plan(const ChunkArgs& a, int heads, int tpt
   return true;
 }
 
-// One partial result in the workspace: CH_ROWS unnormalised output rows, then
-// a (max, sum) pair per row; what it is a part of in a descriptor.  Slot 0 of
+// One partial result in the workspace: CH_ROWS unnormalised output rows, column
+// by column, then a (max, sum) pair per row; what it is a part of in a descriptor.  Slot 0 of
 // a CTA continues an item that an earlier CTA began, slot 1 begins one that a
 // later CTA goes on with.
 struct PartDesc {
@@ -267,17 +271,18 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // ---------------------------------------------------------------------------
 // The kernel.  S = Q K^T and O += P V on the tcgen05 tensor cores, S, P and O
 // in TMEM, K and V in a ring of shared-memory stages.  Warps 0-3 and 4-7 are
-// two softmax warpgroups (A and B) with an S/P and an O accumulator each, one
-// thread a row; warp 8 issues the MMAs; warp 9 loads K and V tiles by TMA and
-// warps 10-11 the queries (pools that TMA cannot read: warps 9-11 load all).
+// two softmax warpgroups (A and B), one thread a row; warp 8 issues the MMAs;
+// warp 9 loads K and V tiles by TMA and warps 10-11 the queries (pools that
+// TMA cannot read: warps 9-15 load all).
 //   more than 128 rows: A and B hold rows 0-127 and 128-255 and every key tile
 //     is used twice;
 //   up to 128 rows: A and B hold the same rows and take the even and the odd
 //     key tiles, joined at the end.
-// While one warpgroup does its softmax the tensor cores work for the other.
-// P overwrites the first half of its S.  O is rescaled only when a row's
-// maximum has grown by more than 2^8 since the last time (weights stay below
-// 2^8, exact in the accumulation's f32); the final division undoes it.
+// While one warpgroup does its softmax the tensor cores work for the other.  A
+// warpgroup takes its 128 scores in halves: the first half's product runs while
+// the second half's weights are computed.  P overwrites the first half of its
+// scores.  O is rescaled only when a row's maximum has grown by more than 2^8
+// since the last time (weights stay below 2^8; the final division undoes it).
 //
 // A V row that the mask hides is weighed with 0, which leaves NaN where it
 // holds infinities or NaN.  Rows behind the last visible key are zeroed in
@@ -306,12 +311,12 @@ struct ChunkSmem {
   static constexpr int STAGES = HD == 128 ? 5 : 8;
   static constexpr int Q = 0, KV = 2 * QTILE, CTRL = KV + STAGES * STAGE;
   // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales
-  static constexpr int BARS = CTRL, PLAN = CTRL + 256, ML = PLAN + 128, QSCALE = ML + 1024;
+  static constexpr int BARS = CTRL, PLAN = CTRL + 320, ML = PLAN + 128, QSCALE = ML + 1024;
   static constexpr int BYTES = QSCALE + 512;
 };
 // barrier numbers
-constexpr int BAR_FULL = 0, BAR_EMPTY = 8, BAR_QFULL = 16, BAR_QEMPTY = 17, BAR_S = 18, BAR_P = 20, BAR_O = 22,
-              BAR_OFREE = 24, BAR_ML = 25, BAR_DRAIN = 26;
+constexpr int BAR_FULL = 0, BAR_EMPTY = 8, BAR_QFULL = 16, BAR_QEMPTY = 17, BAR_OFREE = 18, BAR_ML = 19, BAR_O = 20,
+              BAR_S = 22, BAR_V = 24, BAR_P = 26, BAR_DRAIN = 30;  // P: warpgroup * 2 + half
 
 template <int DT>
 __device__ __forceinline__ float unpack_lo(uint32_t w) {
@@ -335,6 +340,34 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Weights of a row's 64 scores: 2^(c s + nb), stored to TMEM in the products'
+// type, and their f32 sum.  All go to the special-function unit (4 a clock and
+// SM quarter): with 1/8 to 1/2 of them as polynomials on the FMA pipe the
+// softmax was shorter and the whole kernel slower (8192-token prompt 586 us,
+// with a quarter 624 us).
+template <int CT>
+__device__ __forceinline__ float weights(const uint32_t (&v)[CH_HALF], float c, float nb, uint32_t tm_p) {
+  const uint64_t c2 = f32x2(c, c), n2 = f32x2(nb, nb);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int h = 0; h < CH_HALF / 32; ++h) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int k = 32 * h + 2 * i;
+      float e0, e1;
+      f32x2_split(fma_f32x2((uint64_t)v[k + 1] << 32 | v[k], c2, n2), e0, e1);
+      e0 = ex2(e0);
+      e1 = ex2(e1);
+      sum[i & 1] = add_f32x2(sum[i & 1], f32x2(e0, e1));
+      w[i] = pack2<CT>(e0, e1);
+    }
+    tmem_st16(tm_p + 16 * h, w);
+  }
+  float a, b;
+  f32x2_split(add_f32x2(sum[0], sum[1]), a, b);
+  return a + b;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -352,6 +385,16 @@ __device__ __forceinline__ uint32_t kv_off(int r, int c) {
   return (r >> 3) * (HD * 16) + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
+// (scale, zero) pair q of a stored row.
+__device__ __forceinline__ void load_meta(const uint8_t* meta, int q, bool mf32, float& sc, float& zr) {
+  if (mf32) {
+    const float2 m = __ldg(reinterpret_cast<const float2*>(meta) + q);
+    sc = m.x, zr = m.y;
+  } else {
+    const uint32_t m = __ldg(reinterpret_cast<const uint32_t*>(meta) + q);
+    sc = unpack_lo<RMLX_F16>(m), zr = unpack_hi<RMLX_F16>(m);
+  }
+}
 // Eight elements of a stored row as f16 pairs.  w: 8-bit codes in both words,
 // 4-bit codes in w.x.  The group's values lie between zr and zr + qmax sc.
 template <int BITS>
@@ -382,8 +425,38 @@ __device__ __forceinline__ uint4 dequant8(uint2 w, float sc, float zr, bool mf32
   return r;
 }
 
+// Every lane has 64 bytes of a row of its own, going to dst (if valid).  Lanes
+// of a group of four trade 16-byte pieces so that a store instruction writes
+// whole 64-byte runs: a lane a row would write 16 bytes of 32 lines at once.
+__device__ __forceinline__ void store_rows64(uint32_t (&w)[16], uint8_t* dst, bool valid, int lane) {
+  const unsigned long long at = valid ? reinterpret_cast<unsigned long long>(dst) : 0;
+  // transpose the 4 x 4 pieces: exchange blocks of 2, then single ones
+#pragma unroll
+  for (int s = 2; s; s >>= 1) {
+    const bool up = lane & s;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (a & s) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t keep = up ? w[4 * (a | s) + e] : w[4 * a + e], give = up ? w[4 * a + e] : w[4 * (a | s) + e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, s);
+        w[4 * a + e] = up ? got : keep;
+        w[4 * (a | s) + e] = up ? keep : got;
+      }
+    }
+  }
+  // lane 4 g + c now holds piece c of the rows of lanes 4 g .. 4 g + 3
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const unsigned long long row = __shfl_sync(0xffffffffu, at, (lane & 28) | r);
+    if (row)
+      reinterpret_cast<uint4*>(row)[lane & 3] = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
+  }
+}
+
 template <int DT, int HD, int BITS, bool TMA>
-__global__ void __launch_bounds__(CH_THREADS, 1)
+__global__ void __launch_bounds__(ch_threads(TMA), 1)
     chunk_attn_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map, int32_t* err) {
   using S = ChunkSmem<HD>;
   constexpr int CT = BITS ? RMLX_F16 : DT;  // type of the products' operands
@@ -391,15 +464,15 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
   constexpr uint32_t IDESC_S = mma_idesc(CT == RMLX_BF16, 128, CH_KEYS, false);
   constexpr uint32_t IDESC_O = mma_idesc(CT == RMLX_BF16, 128, HD, true);
   constexpr uint32_t TM_S = 0, TM_O = 256;  // TMEM columns: S/P of A and B, then O of A and B
-  constexpr int QWARPS = TMA ? 2 : 3;       // warps that load queries
+  constexpr int QWARPS = TMA ? 2 : 7;       // warps that load queries
   extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms are 1024 bytes
   const uint32_t sb = smem_u32(smem);
   const PoolGeo& g = p.g;
   const ChunkArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto bar = [&](int i) { return sb + S::BARS + 8 * i; };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + 240);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 244);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + 304);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 308);
   ItemIter* plan = reinterpret_cast<ItemIter*>(smem + S::PLAN);
   float2* ml_b = reinterpret_cast<float2*>(smem + S::ML);
   uint8_t* qscale = smem + S::QSCALE;  // [2][CH_ROWS] f32 exponents, by item parity
@@ -407,22 +480,24 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < ST; ++i) {
-      mbar_init(bar(BAR_FULL + i), TMA ? 1 : 3);
+      mbar_init(bar(BAR_FULL + i), TMA ? 1 : QWARPS);
       mbar_init(bar(BAR_EMPTY + i), 1);
     }
     mbar_init(bar(BAR_QFULL), QWARPS);
     mbar_init(bar(BAR_QEMPTY), 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(bar(BAR_S + x), 1);
-      mbar_init(bar(BAR_P + x), 4);
+      mbar_init(bar(BAR_V + x), 1);
       mbar_init(bar(BAR_O + x), 1);
+      mbar_init(bar(BAR_P + 2 * x), 4);
+      mbar_init(bar(BAR_P + 2 * x + 1), 4);
     }
+    mbar_init(bar(BAR_DRAIN), 1);
     mbar_init(bar(BAR_OFREE), 8);
     mbar_init(bar(BAR_ML), 4);
-    mbar_init(bar(BAR_DRAIN), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tmem_alloc(sb + S::BARS + 244, 512);
+  if (warp == 8) tmem_alloc(sb + S::BARS + 308, 512);
   pdl_wait();
   pdl_release();
   PartDesc* desc = p.desc + 2 * blockIdx.x;
@@ -459,7 +534,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         }
         continue;
       }
-      const int mine = two ? nk : (x == 0 ? (nk + 1) / 2 : nk / 2);
+      // half tiles: two a tile, one of the last tile where no key of its second half is visible
+      const bool odd = it.t.hi - (it.t.k_lo + it.k1 - 1) * CH_KEYS <= CH_HALF;
+      const int mine = two ? 2 * nk - odd : 2 * (x == 0 ? (nk + 1) / 2 : nk / 2) - (odd && x == ((nk - 1) & 1));
       const bool active = (two ? 128 * x : 0) + wq * 32 < it.t.rows;
       const int pos = it.t.pos0 + tok;
       const int lim = valid ? max(pos + 1, 0) : INT32_MAX;  // visible keys: low <= key < lim
@@ -467,65 +544,62 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
       float m = -INFINITY, l = 0.0f, c = a.scale_log2;
       bool ok = true;
       for (int j = 0; j < mine; ++j) {
-        if (!(ok = mbar_wait(bar(BAR_S + x), ns & 1, abort_flag, err))) break;
-        ++ns;
+        const int b = j & 1;
+        if (b == 0 && !(ok = mbar_wait(bar(BAR_S + x), ns++ & 1, abort_flag, err))) break;
         if (active) {
           tc_fence_after();
           if (BITS && j == 0) c = a.scale_log2 * __uint_as_float((uint32_t)qscale[(nitem & 1) * CH_ROWS + row] << 23);
-          uint32_t v[128];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, v + 32 * i);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld_wait32(v + 32 * i);
-          const int kb = (it.t.k_lo + it.k0 + (two ? j : 2 * j + x)) * CH_KEYS;
-          if (__any_sync(0xffffffffu, kb + CH_KEYS > lim || kb < low)) {
+          uint32_t v[CH_HALF];
+          tmem_ld32(tm_s + CH_HALF * b, v);
+          tmem_ld32(tm_s + CH_HALF * b + 32, v + 32);
+          const int kb = (it.t.k_lo + it.k0 + (two ? j >> 1 : (j & ~1) + x)) * CH_KEYS + CH_HALF * b;
+          const bool masked = __any_sync(0xffffffffu, kb + CH_HALF > lim || kb < low);
+          tmem_ld_wait32(v);
+          tmem_ld_wait32(v + 32);
+          if (masked) {
             const int r1 = lim - kb, r0 = low - kb;
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
+            for (int i = 0; i < CH_HALF; ++i)
               if (i >= r1 || i < r0) v[i] = 0xff800000u;  // -inf
           }
-          float mx = __uint_as_float(v[0]);
+          float mx4[4];
 #pragma unroll
-          for (int i = 1; i < 128; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+          for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+#pragma unroll
+          for (int i = 8; i < CH_HALF; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx4[k] = fmaxf(mx4[k], fmaxf(__uint_as_float(v[i + 2 * k]), __uint_as_float(v[i + 2 * k + 1])));
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
           if (__any_sync(0xffffffffu, (mx - m) * c > 8.0f)) {
             const float n = fmaxf(m, mx);
             const float f = n == m ? 1.0f : ex2((m - n) * c);
             m = n;
             l *= f;
             if (j > 0) {
+              // products into O have to be done: those of earlier tiles are (these scores were issued
+              // behind them), the tile's first half signals its own
+              if (b && !(ok = mbar_wait(bar(BAR_V + x), (ns - 1) & 1, abort_flag, err))) break;
+              tc_fence_after();
 #pragma unroll 1
-              for (int i = 0; i < HD; i += 32) {
-                uint32_t o[32];
-                tmem_ld32(tm_o + i, o);
-                tmem_ld_wait32(o);
+              for (int i = 0; i < HD; i += 16) {
+                uint32_t o[16];
+                tmem_ld16(tm_o + i, o);
+                tmem_ld_wait16(o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(tm_o + i, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(tm_o + i, o);
               }
               tc_wait_st();
             }
           }
           const float nb = m == -INFINITY ? 0.0f : -m * c;
-          float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float e0 = ex2(fmaf(__uint_as_float(v[64 * h + 2 * i]), c, nb));
-              const float e1 = ex2(fmaf(__uint_as_float(v[64 * h + 2 * i + 1]), c, nb));
-              sum0 += e0;
-              sum1 += e1;
-              w[i] = pack2<CT>(e0, e1);
-            }
-            tmem_st32(tm_s + 32 * h, w);
-          }
-          l += sum0 + sum1;
+          l += weights<CT>(v, c, nb, tm_s + CH_HALF * b);
           tc_wait_st();
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(BAR_P + x));
+        if (lane == 0) mbar_arrive(bar(BAR_P + 2 * x + b));
       }
       if (!ok) break;
       // ---- epilogue ---------------------------------------------------------
@@ -594,18 +668,14 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             f[e] = l == 0.0f ? 0.0f : f[e] * il;
             nan = fmaf(f[e], 0.0f, nan);
           }
-          if (valid) {
-            if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(p.a.out + (orow * HD + i) * 2);
+          if (whole) {
+            uint32_t w[16];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                dst[e] = make_uint4(pack2<DT>(f[8 * e], f[8 * e + 1]), pack2<DT>(f[8 * e + 2], f[8 * e + 3]),
-                                    pack2<DT>(f[8 * e + 4], f[8 * e + 5]), pack2<DT>(f[8 * e + 6], f[8 * e + 7]));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(part + (size_t)row * HD + i);
+            for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(f[2 * e], f[2 * e + 1]);
+            store_rows64(w, p.a.out + (orow * HD + i) * 2, valid, lane);
+          } else if (valid) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-            }
+            for (int e = 0; e < 32; ++e) part[(size_t)(i + e) * CH_ROWS + row] = f[e];  // a warp's lanes side by side
           }
         }
         if (valid && !whole) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[row] = make_float2(ml, l);
@@ -634,7 +704,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             if (whole)
               reinterpret_cast<uint16_t*>(p.a.out)[bo * HD + lane * EPL + e] = (uint16_t)pack2<DT>(y, 0.0f);
             else
-              part[(size_t)br * HD + lane * EPL + e] = y;
+              part[(size_t)(lane * EPL + e) * CH_ROWS + br] = y;
           }
           if (!whole && lane == 0) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[br] = make_float2(bm, bl);
         }
@@ -645,89 +715,103 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     }
   } else if (warp == 8) {
     // ---- MMA issue ----------------------------------------------------------
-    uint32_t n = 0, nitem = 0, np[2] = {0, 0};
+    uint32_t nitem = 0, pp = 0;  // items; a phase bit for each P buffer
+    uint32_t st = 0, ph = 0;     // the ring's next stage and its phase
     bool ok = true;
-    const uint32_t q_base = sb + S::Q, kv_base = sb + S::KV;
-    auto full = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_FULL + i % ST), (i / ST) & 1, abort_flag, err); };
-    auto scores = [&](int x, int qt, uint32_t stage) {  // S_x = Q_qt K^T
-      if (lane == 0) {
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t qd = smem_desc(q_base + qt * S::QTILE + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024);
-          const uint64_t kd = smem_desc(kv_base + stage * S::STAGE + (kk >> 2) * 1024 + (kk & 3) * 32, 16, HD * 16);
-          mma_ss(tmem + TM_S + 128 * x, qd, kd, IDESC_S, kk > 0);
-        }
-        tc_commit(bar(BAR_S + x));
+    auto wait = [&](int b, uint32_t parity) { return ok = ok && mbar_wait(bar(b), parity & 1, abort_flag, err); };
+    auto advance = [&] {
+      if (++st == ST) st = 0, ph ^= 1;
+    };
+    // operand descriptors of the first stage; a stage, or 64 rows, adds its bytes / 16
+    constexpr uint32_t HALF = CH_HALF * HD * 2 / 16;
+    const uint64_t qd = smem_desc(sb + S::Q, 16, 1024), kd = smem_desc(sb + S::KV, 16, HD * 16),
+                   vd = smem_desc(sb + S::KV, 1024, HD * 16);
+    auto scores = [&](int x, int qt, uint32_t stage) {  // S[x] = Q[qt] K^T
+      mma_ss_rows<HD>(tmem + TM_S + 128 * x, qd + (uint32_t)(qt * (S::QTILE / 16)), kd + stage * (S::STAGE / 16), IDESC_S);
+      tc_commit(bar(BAR_S + x));
+    };
+    auto values = [&](int x, uint32_t stage, int h, int keys, bool first) {  // O[x] (+)= P[x][h] V
+      const uint64_t v0 = vd + (stage * (S::STAGE / 16) + h * HALF);
+      const uint32_t o = tmem + TM_O + HD * x, s = tmem + TM_S + 128 * x + CH_HALF * h;
+      if (keys >= CH_HALF - 15) {
+        mma_ts_64<HD>(o, s, v0, IDESC_O, !first);
+      } else {
+        for (int kk = 0; 16 * kk < keys; ++kk) mma_ts_16(o, s + 8 * kk, v0 + kk * (HD * 2), IDESC_O, kk > 0 || !first);
       }
     };
-    auto values = [&](int x, uint32_t stage, int steps, bool first) {  // O_x (+)= P_x V
-      if (lane == 0) {
-        for (int kk = 0; kk < steps; ++kk)
-          mma_ts(tmem + TM_O + HD * x, tmem + TM_S + 128 * x + 8 * kk,
-                 smem_desc(kv_base + stage * S::STAGE + kk * (HD * 32), 1024, HD * 16), IDESC_O, !(first && kk == 0));
-      }
+    auto weights_ready = [&](int x, int h) {
+      if (!wait(BAR_P + 2 * x + h, pp >> (2 * x + h))) return false;
+      pp ^= 1u << (2 * x + h);
+      tc_fence_after();
+      return true;
     };
     for (bool more = next_portion(it, a, g.heads, p.tpt, true); more;
          more = next_portion(it, a, g.heads, p.tpt, false)) {
       const int nk = it.k1 - it.k0;
       if (nk == 0) continue;
       const bool two = it.t.rows > 128;
-      const int lead = two ? 1 : min(2, nk);
-      if (!(ok = mbar_wait(bar(BAR_QFULL), nitem & 1, abort_flag, err))) break;
-      for (int i = 0; i < lead && ok; ++i) {
-        if (!full(n)) break;
-        tc_fence_after();
-        scores(two ? 0 : i, 0, n % ST);
-        if (two) scores(1, 1, n % ST);
-        if (lane == 0) tc_commit(bar(BAR_EMPTY + n % ST));
-        ++n;
-      }
-      if (!ok) break;
-      if (lead == nk && lane == 0) tc_commit(bar(BAR_QEMPTY));
-      for (int j = 0; j < nk; ++j) {
-        const uint32_t sv = n++;  // V of tile j; then K of tile j + lead
-        const bool k_next = j + lead < nk;
-        const uint32_t sk = n;
-        if (k_next) ++n;
-        if (!full(sv)) break;
-        const int keys = min(CH_KEYS, it.t.hi - (it.t.k_lo + it.k0 + j) * CH_KEYS);
-        const int steps = (keys + 15) / 16;
+      auto keys_of = [&](int j) { return min(CH_KEYS, it.t.hi - (it.t.k_lo + it.k0 + j) * CH_KEYS); };
+      auto fill = [&](uint32_t stage, int keys) {
+        // V rows behind the last visible key that share its MMA step: zeros
         if (TMA && (keys & 15)) {
-          // keys behind the last visible one that share its MMA step: zeros
-          for (int i = lane; i < (16 * steps - keys) * (HD / 8); i += 32)
-            sts128(kv_base + (sv % ST) * S::STAGE + kv_off<HD>(keys + i / (HD / 8), i % (HD / 8)), make_uint4(0u, 0u, 0u, 0u));
+          for (int i = lane; i < (16 - (keys & 15)) * (HD / 8); i += 32)
+            sts128(sb + S::KV + stage * S::STAGE + kv_off<HD>(keys + i / (HD / 8), i % (HD / 8)), make_uint4(0u, 0u, 0u, 0u));
           fence_async_smem();
           __syncwarp();
         }
-        if (j == 0 && nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, abort_flag, err))) break;
+      };
+      const int lead = two ? 1 : min(2, nk);
+      if (!wait(BAR_QFULL, nitem)) break;
+      for (int i = 0; i < lead; ++i) {
+        if (!wait(BAR_FULL + st, ph)) break;
+        tc_fence_after();
+        scores(two ? 0 : i, 0, st);
+        if (two) scores(1, 1, st);
+        tc_commit(bar(BAR_EMPTY + st));
+        advance();
+      }
+      if (!ok) break;
+      if (lead == nk) tc_commit(bar(BAR_QEMPTY));
+      if (nitem > 0 && !wait(BAR_OFREE, nitem - 1)) break;
+      for (int j = 0; j < nk; ++j) {
+        const uint32_t sv = st;
+        if (!wait(BAR_FULL + sv, ph)) break;
+        advance();
+        const int keys = keys_of(j), jn = j + lead;
+        fill(sv, keys);
+        const uint32_t sk = st;
+        if (jn < nk) {
+          if (!wait(BAR_FULL + sk, ph)) break;
+          advance();
+        }
         for (int y = 0; y < (two ? 2 : 1); ++y) {
           const int x = two ? y : j & 1;
-          if (!(ok = mbar_wait(bar(BAR_P + x), np[x] & 1, abort_flag, err))) break;
-          ++np[x];
-          tc_fence_after();
-          values(x, sv % ST, steps, two ? j == 0 : j < 2);
-          if (two ? j == nk - 1 : j >= nk - 2)
-            if (lane == 0) tc_commit(bar(BAR_O + x));
-          if (y == (two ? 1 : 0) && lane == 0) tc_commit(bar(BAR_EMPTY + sv % ST));
-          if (k_next) {
-            if (y == 0) {
-              if (!full(sk)) break;
-              tc_fence_after();
-            }
-            scores(x, two ? y : 0, sk % ST);
-            if (y == (two ? 1 : 0) && lane == 0) {
-              tc_commit(bar(BAR_EMPTY + sk % ST));
-              if (j + lead == nk - 1) tc_commit(bar(BAR_QEMPTY));
-            }
+          const bool first = j < lead;
+          if (!weights_ready(x, 0)) break;
+          values(x, sv, 0, keys, first);
+          tc_commit(bar(BAR_V + x));
+          if (keys > CH_HALF) {
+            if (!weights_ready(x, 1)) break;
+            values(x, sv, 1, keys - CH_HALF, false);
+          }
+          if (jn < nk) {
+            scores(x, two ? y : 0, sk);
+          } else {
+            tc_commit(bar(BAR_O + x));
           }
         }
         if (!ok) break;
+        tc_commit(bar(BAR_EMPTY + sv));
+        if (jn < nk) {
+          tc_commit(bar(BAR_EMPTY + sk));
+          if (jn == nk - 1) tc_commit(bar(BAR_QEMPTY));
+        }
       }
       if (!ok) break;
       ++nitem;
     }
     if (!ok) {  // leave no MMA in flight behind
-      if (lane == 0) tc_commit(bar(BAR_DRAIN));
+      tc_commit(bar(BAR_DRAIN));
       for (int i = 0; i < (1 << 20) && !mbar_try(bar(BAR_DRAIN), 0); ++i) {
       }
     }
@@ -737,7 +821,6 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     bool ok = true;
     const bool loads_q = !TMA || warp >= 10, loads_kv = !TMA || warp == 9;
     const int qw = TMA ? warp - 10 : warp - 9;
-    const int64_t vdelta = (int64_t)g.heads * g.tile_bytes;
     for (bool more = next_portion(it, a, g.heads, p.tpt, true); more;
          more = next_portion(it, a, g.heads, p.tpt, false)) {
       const int nk = it.k1 - it.k0;
@@ -749,12 +832,22 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         constexpr int CPR = HD / 8, RPW = 32 / CPR;  // 16-byte chunks of a row, rows of a warp's pass
         const uint8_t* qbase = a.q + (int64_t)(it.qoff + it.t.t0) * a.qts + (int64_t)it.head * a.G * a.qhs;
         const int ch = lane % CPR;
-        constexpr int U = 4;
-        for (int r0 = (qw * RPW) + lane / CPR; r0 < it.t.rows + (int)(lane / CPR); r0 += U * QWARPS * RPW) {
+        const int step = QWARPS * RPW;
+        if (!BITS) {
+          // every row's copy in flight at once
+          for (int r = qw * RPW + lane / CPR; r < it.t.rows; r += step) {
+            const int tok = r / a.G;
+            cp_async16(sb + S::Q + (r >> 7) * S::QTILE + q_off<HD>(r & 127, ch),
+                       qbase + tok * a.qts + (r - tok * a.G) * a.qhs + ch * 16);
+          }
+          cp_async_wait_all();
+        } else {
+        constexpr int U = 8;
+        for (int r0 = (qw * RPW) + lane / CPR; r0 < it.t.rows + (int)(lane / CPR); r0 += U * step) {
           uint4 w[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * QWARPS * RPW;
+            const int r = r0 + u * step;
             w[u] = make_uint4(0u, 0u, 0u, 0u);
             if (r < it.t.rows) {
               const int tok = r / a.G;
@@ -763,8 +856,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * QWARPS * RPW;
-            if (BITS) {
+            const int r = r0 + u * step;
+            {
               // the row's power of two, and a bf16 row in f16
               int e = 127;
               if (DT == RMLX_BF16) {
@@ -787,25 +880,35 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
               sts128(sb + S::Q + (r >> 7) * S::QTILE + q_off<HD>(r & 127, ch), w[u]);
           }
         }
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(BAR_QFULL));
       }
       ++nitem;
       if (!loads_kv) continue;
-      auto load = [&](int j, int kv) {
-        const uint32_t stage = n % ST, dst = sb + S::KV + stage * S::STAGE;
-        if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) return;
-        ++n;
-        const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
-        if constexpr (TMA) {
+      const int lead = two ? 1 : min(2, nk);
+      // loads in the order of their use: K 0 .. lead - 1, then V j and K j + lead
+      const int loads = 2 * nk;
+      auto which = [&](int i, int& j, int& kv) {
+        if (i < lead) j = i, kv = 0;
+        else if (i - lead >= 2 * (nk - lead)) j = i - nk, kv = 1;  // the last ones are all V
+        else j = (i - lead) >> 1, kv = ((i - lead) & 1) ^ 1, j += kv ? 0 : lead;
+      };
+      if constexpr (TMA) {
+        for (int i = 0; i < loads; ++i) {
+          int j, kv;
+          which(i, j, kv);
+          const uint32_t stage = n % ST, dst = sb + S::KV + stage * S::STAGE;
+          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
+          ++n;
           // one box of p.box rows a lane
-          const int t = kb + lane * p.box;
+          const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS, t = kb + lane * p.box;
           const bool want = lane * p.box < CH_KEYS && t < it.t.hi;
           int blk = 0, b = 0;
           if (want) {
             b = t / g.bs;
-            blk = b < a.bt_stride ? __ldg(btrow + b) : -1;
+            blk = __ldg(btrow + b);
             if (blk < 0 || blk >= g.nblocks) {
               atomicOr(err, DEV_ERR_BLOCK);
               blk = 0;
@@ -819,60 +922,79 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                         (int)((((int64_t)blk * g.layers + a.layer) * 2 + kv) * g.heads + it.head) * (g.bs / 8) +
                             (t - b * g.bs) / 8,
                         bar(BAR_FULL + stage));
-        } else {
-          // units of 8 elements (plain) or of one 16-byte run of codes
-          constexpr int UPR = BITS ? HD * BITS / 128 : HD / 8;
-          for (int u = (warp - 9) * 32 + lane; u < CH_KEYS * UPR; u += 96) {
-            const int r = u / UPR, ch = u % UPR, t = kb + r;
-            const uint8_t* tile = nullptr;
-            int slot = 0;
-            if (t < it.t.hi) {
-              const int b = t / g.bs;
-              const int32_t blk = b < a.bt_stride ? __ldg(btrow + b) : -1;
-              if (blk < 0 || blk >= g.nblocks) atomicOr(err, DEV_ERR_BLOCK);
-              else tile = g.base + g.tile_off(blk, a.layer, 0, it.head) + kv * vdelta;
-              slot = t - b * g.bs;
-            }
-            if (!BITS) {
-              uint4 w = make_uint4(0u, 0u, 0u, 0u);
-              if (tile) w = ld_stream(tile + (int64_t)slot * g.row_bytes + ch * 16);
-              sts128(dst + kv_off<HD>(r, ch), w);
-            } else {
-              constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8;  // elements of a unit
-              uint4 w = make_uint4(0u, 0u, 0u, 0u);
-              if (tile) w = ld_stream(tile + (int64_t)slot * g.row_bytes + ch * 16);
-              const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
-              const uint8_t* meta = tile + (int64_t)g.bs * g.row_bytes + (int64_t)slot * g.meta_row_bytes;
-              float sc = 0.0f, zr = 0.0f;
-              int cur = -1;
+        }
+      } else {
+        // A unit is 16 bytes of a stored row: 8 elements, or 16 or 32 codes.  The
+        // next tile's units are in flight while this one's are converted.
+        constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8, UPR = HD / EPU;
+        constexpr int N = (CH_KEYS * UPR + 32 * QWARPS - 1) / (32 * QWARPS);
+        struct Units {
+          uint4 w[N];
+          float sc[N], zr[N];  // of the unit's first group
+          const uint8_t* meta[N];
+        };
+        auto fetch = [&](int i, Units& r) {
+          int j, kv;
+          which(i, j, kv);
+          const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
 #pragma unroll
-              for (int i = 0; i < EPU / 8; ++i) {
-                const int q = (ch * EPU + 8 * i) >> a.gs_log2;
-                if (tile && q != cur) {
-                  cur = q;
-                  if (a.mf32) {
-                    const float2 m2 = __ldg(reinterpret_cast<const float2*>(meta) + q);
-                    sc = m2.x, zr = m2.y;
-                  } else {
-                    const uint32_t m2 = __ldg(reinterpret_cast<const uint32_t*>(meta) + q);
-                    sc = unpack_lo<RMLX_F16>(m2), zr = unpack_hi<RMLX_F16>(m2);
-                  }
+          for (int y = 0; y < N; ++y) {
+            const int u = (y * QWARPS + qw) * 32 + lane, t = kb + u / UPR, ch = u % UPR;
+            r.w[y] = make_uint4(0u, 0u, 0u, 0u);
+            r.sc[y] = r.zr[y] = 0.0f;
+            r.meta[y] = nullptr;
+            if (u < CH_KEYS * UPR && t < it.t.hi) {
+              const int b = a.bs_log2 >= 0 ? t >> a.bs_log2 : t / g.bs, slot = t - b * g.bs;
+              const int32_t blk = __ldg(btrow + b);
+              if (blk < 0 || blk >= g.nblocks) {
+                atomicOr(err, DEV_ERR_BLOCK);
+              } else {
+                const uint8_t* tile = g.base + g.tile_off(blk, a.layer, kv, it.head);
+                r.w[y] = ld_stream(tile + slot * g.row_bytes + ch * 16);
+                if (BITS) {
+                  r.meta[y] = tile + g.bs * g.row_bytes + slot * g.meta_row_bytes;
+                  load_meta(r.meta[y], (ch * EPU) >> a.gs_log2, a.mf32, r.sc[y], r.zr[y]);
                 }
-                const uint2 two8 = BITS == 8 ? make_uint2(cw[2 * (i & 1)], cw[2 * (i & 1) + 1]) : make_uint2(cw[i & 3], 0u);
-                sts128(dst + kv_off<HD>(r, ch * (EPU / 8) + i), dequant8<BITS ? BITS : 8>(two8, sc, zr, a.mf32, kv));
               }
             }
           }
+        };
+        auto put = [&](int i, const Units& r, uint32_t dst) {
+          int j, kv;
+          which(i, j, kv);
+#pragma unroll
+          for (int y = 0; y < N; ++y) {
+            const int u = (y * QWARPS + qw) * 32 + lane, row = u / UPR, ch = u % UPR;
+            if (u >= CH_KEYS * UPR) continue;
+            if constexpr (BITS == 0) {
+              sts128(dst + kv_off<HD>(row, ch), r.w[y]);
+            } else {
+              const uint32_t cw[4] = {r.w[y].x, r.w[y].y, r.w[y].z, r.w[y].w};
+              float sc = r.sc[y], zr = r.zr[y];
+              int cur = (ch * EPU) >> a.gs_log2;
+#pragma unroll
+              for (int e = 0; e < EPU / 8; ++e) {
+                const int q = (ch * EPU + 8 * e) >> a.gs_log2;
+                if (q != cur && r.meta[y]) load_meta(r.meta[y], cur = q, a.mf32, sc, zr);
+                const uint2 c8 = BITS == 8 ? make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]) : make_uint2(cw[e], 0u);
+                sts128(dst + kv_off<HD>(row, ch * (EPU / 8) + e), dequant8<BITS ? BITS : 8>(c8, sc, zr, a.mf32, kv));
+              }
+            }
+          }
+        };
+        Units cur, next;
+        fetch(0, cur);
+        for (int i = 0; i < loads; ++i) {
+          if (i + 1 < loads) fetch(i + 1, next);
+          const uint32_t stage = n % ST;
+          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
+          ++n;
+          put(i, cur, sb + S::KV + stage * S::STAGE);
           fence_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(BAR_FULL + stage));
+          cur = next;
         }
-      };
-      const int lead = two ? 1 : min(2, nk);
-      for (int i = 0; i < lead && ok; ++i) load(i, 0);
-      for (int j = 0; j < nk && ok; ++j) {
-        load(j, 1);
-        if (ok && j + lead < nk) load(j + lead, 0);
       }
       if (!ok) break;
     }
@@ -887,38 +1009,42 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
 }
 
 // Joins the portions of the items that more than one CTA worked on.  Block
-// (c, y): rows 32 y .. of the item that CTA c began and others went on with.
+// (c, y): rows 32 y .. of the item that CTA c began and others went on with,
+// a lane a row, a warp 1 / 8 of the columns.
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) chunk_combine_kernel(ChunkParams p, int nparts) {
-  constexpr int EPL = HD / 32;
+  constexpr int COLS = HD / 8;
   pdl_release();
   pdl_wait();
   const PartDesc d = p.desc[2 * blockIdx.x + 1];
-  if (!d.valid || (int)blockIdx.y * 32 >= d.rows) return;
+  const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) * COLS, row = blockIdx.y * 32 + lane;
+  if (!d.valid || row >= d.rows) return;
   int end = blockIdx.x + 1;  // CTAs c + 1 .. end hold the rest
   while (end < nparts - 1 && !p.desc[2 * end].last) ++end;
-  const int lane = threadIdx.x & 31;
-  for (int row = blockIdx.y * 32 + (threadIdx.x >> 5); row < min(d.rows, (int)blockIdx.y * 32 + 32); row += 8) {
-    float m = -INFINITY, l = 0.0f, acc[EPL];
+  float m = -INFINITY, l = 0.0f, acc[COLS];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) acc[e] = 0.0f;
-    for (int c = blockIdx.x; c <= end; ++c) {
-      const float* part = p.parts + (size_t)(2 * c + (c == (int)blockIdx.x)) * part_floats(HD);
-      const float2 x = __ldcg(reinterpret_cast<const float2*>(part + (size_t)CH_ROWS * HD) + row);
-      const float n = fmaxf(m, x.x), base = n == -INFINITY ? 0.0f : n;
-      const float f0 = ex2(m - base), f1 = ex2(x.x - base);
-      m = n;
-      l = l * f0 + x.y * f1;
+  for (int e = 0; e < COLS; ++e) acc[e] = 0.0f;
+  for (int c = blockIdx.x; c <= end; ++c) {
+    const float* part = p.parts + (size_t)(2 * c + (c == (int)blockIdx.x)) * part_floats(HD);
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(part + (size_t)CH_ROWS * HD) + row);
+    float o[COLS];
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) acc[e] = acc[e] * f0 + __ldcg(part + (size_t)row * HD + lane * EPL + e) * f1;
-    }
-    const float il = l == 0.0f ? 0.0f : 1.0f / l;
-    const int tok = row / p.a.G, gq = row - tok * p.a.G;
-    uint32_t* o = reinterpret_cast<uint32_t*>(
-        p.a.out + (((int64_t)(d.token0 + tok) * p.g.heads + d.head) * p.a.G + gq) * HD * 2 + lane * EPL * 2);
+    for (int e = 0; e < COLS; ++e) o[e] = __ldcg(part + (size_t)(col + e) * CH_ROWS + row);
+    const float n = fmaxf(m, x.x), base = n == -INFINITY ? 0.0f : n;
+    const float f0 = ex2(m - base), f1 = ex2(x.x - base);
+    m = n;
+    l = l * f0 + x.y * f1;
 #pragma unroll
-    for (int e = 0; e < EPL; e += 2) o[e / 2] = pack2<DT>(acc[e] * il, acc[e + 1] * il);
+    for (int e = 0; e < COLS; ++e) acc[e] = acc[e] * f0 + o[e] * f1;
   }
+  const float il = l == 0.0f ? 0.0f : 1.0f / l;
+  const int tok = row / p.a.G, gq = row - tok * p.a.G;
+  uint4* o = reinterpret_cast<uint4*>(
+      p.a.out + ((((int64_t)(d.token0 + tok) * p.g.heads + d.head) * p.a.G + gq) * HD + col) * 2);
+#pragma unroll
+  for (int e = 0; e < COLS / 8; ++e)
+    o[e] = make_uint4(pack2<DT>(acc[8 * e] * il, acc[8 * e + 1] * il), pack2<DT>(acc[8 * e + 2] * il, acc[8 * e + 3] * il),
+                      pack2<DT>(acc[8 * e + 4] * il, acc[8 * e + 5] * il), pack2<DT>(acc[8 * e + 6] * il, acc[8 * e + 7] * il));
 }
 
 }  // namespace rmlx
@@ -1010,6 +1136,7 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   a.qts = qts, a.qhs = qhs;
   a.layer = layer, a.G = q_heads_per_kv, a.bt_stride = block_table_stride, a.nseq = num_seqs, a.nq = num_q_tokens;
   a.window = window;
+  a.bs_log2 = is_pow2(c.block_size) ? log2i(c.block_size) : -1;
   a.max_len = (int)std::min<int64_t>((int64_t)block_table_stride * c.block_size, 1 << 30);
   a.gs_log2 = c.quant_bits ? log2i(c.group_size) : 0, a.bits = c.quant_bits, a.mf32 = c.meta_dtype == RMLX_F32;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;  // log2(e)
@@ -1030,7 +1157,7 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
                                  : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
   const size_t smem = c.head_dim == 128 ? ChunkSmem<128>::BYTES : ChunkSmem<64>::BYTES;
   if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
-  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(CH_THREADS), smem, (cudaStream_t)stream, prm, map, p->err);
+  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(ch_threads(tma)), smem, (cudaStream_t)stream, prm, map, p->err);
   if (e != cudaSuccess) return cuda_check(e, "chunk attention launch");
   auto fc = c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
                               : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>);
