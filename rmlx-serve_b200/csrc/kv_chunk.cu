@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <numeric>
+#include <type_traits>
 
 #include "dequant.cuh"
 #include "kv_pool_internal.cuh"
@@ -303,13 +304,16 @@ struct ChunkParams {
   PartDesc* desc;
 };
 
-template <int HD>
+template <int HD, int BITS>
 struct ChunkSmem {
-  static constexpr int HALVES = HD / 64;
   static constexpr int QTILE = 128 * HD * 2;
   static constexpr int STAGE = CH_KEYS * HD * 2;
-  static constexpr int STAGES = HD == 128 ? 5 : 8;
-  static constexpr int Q = 0, KV = 2 * QTILE, CTRL = KV + STAGES * STAGE;
+  // Quantised pools give two stages up for codes in flight (RAW): 3 tiles of
+  // 16-byte units of 8-bit codes with f16 scales, or 4 of 4-bit codes.
+  static constexpr int STAGES = BITS ? (HD == 128 ? 3 : 6) : HD == 128 ? 5 : 8;
+  static constexpr int UNITS = BITS ? CH_KEYS * HD * BITS / 128 : 0;  // of a tile
+  static constexpr int RAW_BYTES = BITS == 8 ? UNITS * 60 : UNITS * 96;
+  static constexpr int Q = 0, KV = 2 * QTILE, RAW = KV + STAGES * STAGE, CTRL = RAW + RAW_BYTES;
   // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales
   static constexpr int BARS = CTRL, PLAN = CTRL + 320, ML = PLAN + 128, QSCALE = ML + 1024;
   static constexpr int BYTES = QSCALE + 512;
@@ -368,6 +372,21 @@ __device__ __forceinline__ float weights(const uint32_t (&v)[CH_HALF], float c, 
   f32x2_split(add_f32x2(sum[0], sum[1]), a, b);
   return a + b;
 }
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -385,44 +404,54 @@ __device__ __forceinline__ uint32_t kv_off(int r, int c) {
   return (r >> 3) * (HD * 16) + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// (scale, zero) pair q of a stored row.
-__device__ __forceinline__ void load_meta(const uint8_t* meta, int q, bool mf32, float& sc, float& zr) {
-  if (mf32) {
-    const float2 m = __ldg(reinterpret_cast<const float2*>(meta) + q);
-    sc = m.x, zr = m.y;
-  } else {
-    const uint32_t m = __ldg(reinterpret_cast<const uint32_t*>(meta) + q);
-    sc = unpack_lo<RMLX_F16>(m), zr = unpack_hi<RMLX_F16>(m);
-  }
+// (scale, zero) pair q of a stored row, as it lies in memory (f16: in one word).
+__device__ __forceinline__ uint2 load_meta(const uint8_t* meta, int q, bool mf32) {
+  if (mf32) return __ldg(reinterpret_cast<const uint2*>(meta) + q);
+  return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(meta) + q), 0u);
 }
-// Eight elements of a stored row as f16 pairs.  w: 8-bit codes in both words,
-// 4-bit codes in w.x.  The group's values lie between zr and zr + qmax sc.
+// A group's scale and zero as the conversion takes them.  Its values lie
+// between zr and zr + qmax sc: where they leave f16's range, or where V's are
+// so small that f16 would lose their digits, the scale becomes NaN, and the
+// rows that see them take the exact path.
 template <int BITS>
-__device__ __forceinline__ uint4 dequant8(uint2 w, float sc, float zr, bool mf32, bool is_v) {
-  const float ma = fmaxf(fabsf(zr), fabsf(fmaf((float)((1 << BITS) - 1), sc, zr)));
-  if (!(ma <= 65504.0f) || (is_v && ma > 0.0f && ma < 3.0517578125e-5f)) sc = __uint_as_float(0x7fffffffu);
+struct Group {
+  float sc, zr;
+  __half2 sc2, zr2;
+  __device__ __forceinline__ void set(uint2 meta, bool mf32, bool is_v) {
+    float s = mf32 ? __uint_as_float(meta.x) : unpack_lo<RMLX_F16>(meta.x);
+    const float z = mf32 ? __uint_as_float(meta.y) : unpack_hi<RMLX_F16>(meta.x);
+    const float top = fmaxf(fabsf(z), fabsf(fmaf((float)((1 << BITS) - 1), s, z)));
+    if (!(top <= 65504.0f) || (is_v && top > 0.0f && top < 3.0517578125e-5f)) s = __uint_as_float(0x7fffffffu);
+    sc = s, zr = z;
+    sc2 = __float2half2_rn(s), zr2 = __float2half2_rn(z);
+  }
+};
+// Eight elements as f16 pairs from their codes, a byte each.  A code becomes
+// the f16 1024 + code by a byte permute, then code exactly; f16 scale and
+// zero give code * scale + zero with one rounding, f32 ones with one of f32 more.
+template <int BITS, bool MF32>
+__device__ __forceinline__ uint4 dequant8(uint2 w, const Group<BITS>& g) {
   uint4 r;
   uint32_t* o = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t m;  // two codes as f16 1024 + code
-    if (BITS == 8) {
-      m = __byte_perm(i < 2 ? w.x : w.y, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
-    } else {
-      const uint32_t b = w.x >> (8 * i);
-      m = 0x64006400u | (b & 15) | ((b & 0xf0) << 12);
-    }
-    const __half2 c = __hsub2(*reinterpret_cast<__half2*>(&m), __floats2half2_rn(1024.0f, 1024.0f));
+    const uint32_t m = __byte_perm(i < 2 ? w.x : w.y, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
+    const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1024.0f, 1024.0f));
     __half2 v;
-    if (mf32) {
+    if (MF32) {
       const float2 f = __half22float2(c);
-      v = __floats2half2_rn(fmaf(f.x, sc, zr), fmaf(f.y, sc, zr));
-    } else {  // f16 scale and zero: one rounding
-      v = __hfma2(c, __float2half2_rn(sc), __float2half2_rn(zr));
+      v = __floats2half2_rn(fmaf(f.x, g.sc, g.zr), fmaf(f.y, g.sc, g.zr));
+    } else {
+      v = __hfma2(c, g.sc2, g.zr2);
     }
     o[i] = *reinterpret_cast<uint32_t*>(&v);
   }
   return r;
+}
+// Eight 4-bit codes, low nibble first, as bytes.
+__device__ __forceinline__ uint2 nibbles(uint32_t w) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+  return make_uint2(__byte_perm(lo, hi, 0x5140), __byte_perm(lo, hi, 0x7362));
 }
 
 // Every lane has 64 bytes of a row of its own, going to dst (if valid).  Lanes
@@ -458,7 +487,7 @@ __device__ __forceinline__ void store_rows64(uint32_t (&w)[16], uint8_t* dst, bo
 template <int DT, int HD, int BITS, bool TMA>
 __global__ void __launch_bounds__(ch_threads(TMA), 1)
     chunk_attn_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map, int32_t* err) {
-  using S = ChunkSmem<HD>;
+  using S = ChunkSmem<HD, BITS>;
   constexpr int CT = BITS ? RMLX_F16 : DT;  // type of the products' operands
   constexpr int ST = S::STAGES;
   constexpr uint32_t IDESC_S = mma_idesc(CT == RMLX_BF16, 128, CH_KEYS, false);
@@ -924,77 +953,124 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
                         bar(BAR_FULL + stage));
         }
       } else {
-        // A unit is 16 bytes of a stored row: 8 elements, or 16 or 32 codes.  The
-        // next tile's units are in flight while this one's are converted.
-        constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8, UPR = HD / EPU;
-        constexpr int N = (CH_KEYS * UPR + 32 * QWARPS - 1) / (32 * QWARPS);
-        struct Units {
-          uint4 w[N];
-          float sc[N], zr[N];  // of the unit's first group
-          const uint8_t* meta[N];
-        };
-        auto fetch = [&](int i, Units& r) {
+        // A unit is 16 bytes of a stored row: 8 elements, or 16 or 32 codes.  Rows
+        // go straight into their stage; codes, with the scale and zero of a unit's
+        // first group, into a ring of their own, from which the thread that
+        // copied them converts them `depth` - 1 loads later (with registers
+        // instead of the ring one tile was in flight: 4-bit chunks 290 us).
+        constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8, UPR = HD / EPU, UNITS = CH_KEYS * UPR;
+        constexpr int N = (UNITS + 32 * QWARPS - 1) / (32 * QWARPS);
+        const int depth = BITS == 0 ? 3 : BITS == 4 ? 4 : a.mf32 ? 2 : 3;
+        const int ch = lane % UPR;  // the same for all of a lane's units
+        const int64_t block_bytes = (int64_t)g.layers * 2 * g.heads * g.tile_bytes;
+        const uint8_t* head_base = g.base + g.tile_off(0, a.layer, 0, it.head);
+        const int u0 = qw * 32 + lane;
+        const uint32_t raw_meta = sb + S::RAW + depth * UNITS * 16;
+        auto key_of = [&](int j, int y) { return (it.t.k_lo + it.k0 + j) * CH_KEYS + (u0 + y * QWARPS * 32) / UPR; };
+        // block ids of a load's units, a load ahead of the units themselves
+        auto fetch_ids = [&](int i, int32_t (&blk)[N]) {
           int j, kv;
           which(i, j, kv);
-          const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
 #pragma unroll
           for (int y = 0; y < N; ++y) {
-            const int u = (y * QWARPS + qw) * 32 + lane, t = kb + u / UPR, ch = u % UPR;
-            r.w[y] = make_uint4(0u, 0u, 0u, 0u);
-            r.sc[y] = r.zr[y] = 0.0f;
-            r.meta[y] = nullptr;
-            if (u < CH_KEYS * UPR && t < it.t.hi) {
-              const int b = a.bs_log2 >= 0 ? t >> a.bs_log2 : t / g.bs, slot = t - b * g.bs;
-              const int32_t blk = __ldg(btrow + b);
-              if (blk < 0 || blk >= g.nblocks) {
-                atomicOr(err, DEV_ERR_BLOCK);
-              } else {
-                const uint8_t* tile = g.base + g.tile_off(blk, a.layer, kv, it.head);
-                r.w[y] = ld_stream(tile + slot * g.row_bytes + ch * 16);
-                if (BITS) {
-                  r.meta[y] = tile + g.bs * g.row_bytes + slot * g.meta_row_bytes;
-                  load_meta(r.meta[y], (ch * EPU) >> a.gs_log2, a.mf32, r.sc[y], r.zr[y]);
-                }
-              }
-            }
+            const int t = key_of(j, y);
+            blk[y] = -1;
+            if (u0 + y * QWARPS * 32 < UNITS && t < it.t.hi) blk[y] = __ldg(btrow + (a.bs_log2 >= 0 ? t >> a.bs_log2 : t / g.bs));
           }
         };
-        auto put = [&](int i, const Units& r, uint32_t dst) {
+        auto copy = [&](int i, const int32_t (&blk)[N], uint32_t stage, int slot) {
           int j, kv;
           which(i, j, kv);
+          const uint8_t* base = head_base + (kv ? (int64_t)g.heads * g.tile_bytes : 0);
 #pragma unroll
           for (int y = 0; y < N; ++y) {
-            const int u = (y * QWARPS + qw) * 32 + lane, row = u / UPR, ch = u % UPR;
-            if (u >= CH_KEYS * UPR) continue;
-            if constexpr (BITS == 0) {
-              sts128(dst + kv_off<HD>(row, ch), r.w[y]);
+            const int u = u0 + y * QWARPS * 32;
+            if (u >= UNITS) continue;
+            const int t = key_of(j, y), r = a.bs_log2 >= 0 ? t & (g.bs - 1) : t % g.bs;
+            const bool good = t < it.t.hi && blk[y] >= 0 && blk[y] < g.nblocks;  // else zeros
+            if (t < it.t.hi && !good) atomicOr(err, DEV_ERR_BLOCK);
+            const uint8_t* tile = good ? base + blk[y] * block_bytes : g.base;
+            if (BITS == 0) {
+              cp_async16_zfill(sb + S::KV + stage * S::STAGE + kv_off<HD>(u / UPR, ch), good ? tile + r * g.row_bytes + ch * 16 : tile, good);
             } else {
-              const uint32_t cw[4] = {r.w[y].x, r.w[y].y, r.w[y].z, r.w[y].w};
-              float sc = r.sc[y], zr = r.zr[y];
-              int cur = (ch * EPU) >> a.gs_log2;
-#pragma unroll
-              for (int e = 0; e < EPU / 8; ++e) {
-                const int q = (ch * EPU + 8 * e) >> a.gs_log2;
-                if (q != cur && r.meta[y]) load_meta(r.meta[y], cur = q, a.mf32, sc, zr);
-                const uint2 c8 = BITS == 8 ? make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]) : make_uint2(cw[e], 0u);
-                sts128(dst + kv_off<HD>(row, ch * (EPU / 8) + e), dequant8<BITS ? BITS : 8>(c8, sc, zr, a.mf32, kv));
-              }
+              cp_async16_zfill(sb + S::RAW + (slot * UNITS + u) * 16, good ? tile + r * g.row_bytes + ch * 16 : tile, good);
+              const int q = (ch * EPU) >> a.gs_log2;
+              const uint8_t* meta = good ? tile + g.bs * g.row_bytes + r * g.meta_row_bytes + q * (a.mf32 ? 8 : 4) : g.base;
+              if (a.mf32) cp_async_zfill<8>(raw_meta + (slot * UNITS + u) * 8, meta, good);
+              else cp_async_zfill<4>(raw_meta + (slot * UNITS + u) * 4, meta, good);
             }
           }
         };
-        Units cur, next;
-        fetch(0, cur);
-        for (int i = 0; i < loads; ++i) {
-          if (i + 1 < loads) fetch(i + 1, next);
-          const uint32_t stage = n % ST;
-          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
-          ++n;
-          put(i, cur, sb + S::KV + stage * S::STAGE);
+        // mf32: f32 scales and zeros; one: a unit's elements are all of one group
+        auto convert_as = [&](int i, uint32_t stage, int slot, auto mf32, auto one) {
+          constexpr bool MF32 = decltype(mf32)::value;
+          int j, kv;
+          which(i, j, kv);
+#pragma unroll
+          for (int y = 0; y < N; ++y) {
+            const int u = u0 + y * QWARPS * 32;
+            if (u >= UNITS) continue;
+            const uint4 w = lds128(sb + S::RAW + (slot * UNITS + u) * 16);
+            const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
+            Group<BITS ? BITS : 8> grp;
+            grp.set(MF32 ? lds64(raw_meta + (slot * UNITS + u) * 8) : make_uint2(lds32(raw_meta + (slot * UNITS + u) * 4), 0u),
+                    MF32, kv);
+            const uint8_t* meta = nullptr;
+            if (!decltype(one)::value) {
+              const int t = key_of(j, y);
+              const int b = a.bs_log2 >= 0 ? t >> a.bs_log2 : t / g.bs;
+              const int32_t blk = t < it.t.hi ? __ldg(btrow + b) : -1;
+              if (blk >= 0 && blk < g.nblocks)
+                meta = head_base + (kv ? (int64_t)g.heads * g.tile_bytes : 0) + blk * block_bytes + g.bs * g.row_bytes +
+                       (t - b * g.bs) * g.meta_row_bytes;
+            }
+            uint4 o[EPU / 8];
+#pragma unroll
+            for (int e = 0; e < EPU / 8; ++e) {
+              if (!decltype(one)::value && e > 0 && meta)
+                grp.set(load_meta(meta, (ch * EPU + 8 * e) >> a.gs_log2, MF32), MF32, kv);
+              o[e] = dequant8<BITS ? BITS : 8, MF32>(
+                  BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
+            }
+#pragma unroll
+            for (int e = 0; e < EPU / 8; ++e)
+              sts128(sb + S::KV + stage * S::STAGE + kv_off<HD>(u / UPR, ch * (EPU / 8) + e), o[e]);
+          }
+        };
+        auto convert = [&](int i, uint32_t stage, int slot) {
+          const bool one = (1 << a.gs_log2) >= EPU;
+          if (!a.mf32 && one) convert_as(i, stage, slot, std::false_type(), std::true_type());
+          else if (!a.mf32) convert_as(i, stage, slot, std::false_type(), std::false_type());
+          else if (one) convert_as(i, stage, slot, std::true_type(), std::true_type());
+          else convert_as(i, stage, slot, std::true_type(), std::false_type());
+        };
+        auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, abort_flag, err); };
+        int32_t ids[N];
+        fetch_ids(0, ids);
+        int in = 0, out = 0;  // ring slots of the next copy and the next conversion
+        for (int i = 0; i < loads + depth - 1; ++i) {
+          if (i < loads) {
+            if (BITS == 0 && !empty(n + i)) break;
+            copy(i, ids, (n + i) % ST, in);
+            if (++in == depth) in = 0;
+            if (i + 1 < loads) fetch_ids(i + 1, ids);
+          }
+          cp_async_commit();
+          const int d = i - (depth - 1);
+          if (d < 0) continue;
+          if (depth == 2) cp_async_wait<1>();
+          else if (depth == 3) cp_async_wait<2>();
+          else cp_async_wait<3>();
+          if (BITS != 0) {
+            if (!empty(n + d)) break;
+            convert(d, (n + d) % ST, out);
+            if (++out == depth) out = 0;
+          }
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(BAR_FULL + stage));
-          cur = next;
+          if (lane == 0) mbar_arrive(bar(BAR_FULL + (n + d) % ST));
         }
+        n += loads;
       }
       if (!ok) break;
     }
@@ -1059,6 +1135,11 @@ ChunkFn pick_chunk(int bits, bool tma) {
   if (bits == 8) return chunk_attn_kernel<DT, HD, 8, false>;
   if (bits == 4) return chunk_attn_kernel<DT, HD, 4, false>;
   return tma ? chunk_attn_kernel<DT, HD, 0, true> : chunk_attn_kernel<DT, HD, 0, false>;
+}
+
+template <int HD>
+size_t chunk_smem(int bits) {
+  return bits == 8 ? ChunkSmem<HD, 8>::BYTES : bits == 4 ? ChunkSmem<HD, 4>::BYTES : ChunkSmem<HD, 0>::BYTES;
 }
 
 size_t chunk_workspace(const rmlx_kv_pool* p) {
@@ -1155,7 +1236,7 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   if (tma && (s = chunk_map(p, prm.box, &map)) != RMLX_OK) return s;
   ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
                                  : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
-  const size_t smem = c.head_dim == 128 ? ChunkSmem<128>::BYTES : ChunkSmem<64>::BYTES;
+  const size_t smem = c.head_dim == 128 ? chunk_smem<128>(c.quant_bits) : chunk_smem<64>(c.quant_bits);
   if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
   cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(ch_threads(tma)), smem, (cudaStream_t)stream, prm, map, p->err);
   if (e != cudaSuccess) return cuda_check(e, "chunk attention launch");
