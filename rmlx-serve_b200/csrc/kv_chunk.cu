@@ -967,37 +967,45 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         const int u0 = qw * 32 + lane;
         const uint32_t raw_meta = sb + S::RAW + depth * UNITS * 16;
         auto key_of = [&](int j, int y) { return (it.t.k_lo + it.k0 + j) * CH_KEYS + (u0 + y * QWARPS * 32) / UPR; };
-        // block ids of a load's units, a load ahead of the units themselves
-        auto fetch_ids = [&](int i, int32_t (&blk)[N]) {
+        // block ids (-1: no row) and rows in them of a load's units, a load ahead of the units themselves
+        auto fetch_ids = [&](int i, int32_t (&blk)[N], int32_t (&row)[N]) {
           int j, kv;
           which(i, j, kv);
+          int b[N];
+          if (a.bs_log2 >= 0) {
+#pragma unroll
+            for (int y = 0; y < N; ++y) b[y] = key_of(j, y) >> a.bs_log2, row[y] = key_of(j, y) & (g.bs - 1);
+          } else {
+#pragma unroll
+            for (int y = 0; y < N; ++y) b[y] = key_of(j, y) / g.bs, row[y] = key_of(j, y) - b[y] * g.bs;
+          }
 #pragma unroll
           for (int y = 0; y < N; ++y) {
-            const int t = key_of(j, y);
             blk[y] = -1;
-            if (u0 + y * QWARPS * 32 < UNITS && t < it.t.hi) blk[y] = __ldg(btrow + (a.bs_log2 >= 0 ? t >> a.bs_log2 : t / g.bs));
+            if (u0 + y * QWARPS * 32 < UNITS && key_of(j, y) < it.t.hi) blk[y] = __ldg(btrow + b[y]);
           }
         };
-        auto copy = [&](int i, const int32_t (&blk)[N], uint32_t stage, int slot) {
+        // straight-line, so that the units' address arithmetic overlaps
+        bool bad = false;
+        auto copy = [&](int i, const int32_t (&blk)[N], const int32_t (&row)[N], uint32_t stage, int slot) {
           int j, kv;
           which(i, j, kv);
           const uint8_t* base = head_base + (kv ? (int64_t)g.heads * g.tile_bytes : 0);
 #pragma unroll
           for (int y = 0; y < N; ++y) {
             const int u = u0 + y * QWARPS * 32;
-            if (u >= UNITS) continue;
-            const int t = key_of(j, y), r = a.bs_log2 >= 0 ? t & (g.bs - 1) : t % g.bs;
-            const bool good = t < it.t.hi && blk[y] >= 0 && blk[y] < g.nblocks;  // else zeros
-            if (t < it.t.hi && !good) atomicOr(err, DEV_ERR_BLOCK);
-            const uint8_t* tile = good ? base + blk[y] * block_bytes : g.base;
+            const bool unit = u < UNITS, want = unit && key_of(j, y) < it.t.hi;
+            const bool good = want && (uint32_t)blk[y] < (uint32_t)g.nblocks;  // else zeros
+            bad |= want && !good;
+            const uint8_t* tile = base + (good ? blk[y] : 0) * block_bytes;
             if (BITS == 0) {
-              cp_async16_zfill(sb + S::KV + stage * S::STAGE + kv_off<HD>(u / UPR, ch), good ? tile + r * g.row_bytes + ch * 16 : tile, good);
+              cp_async16_zfill(sb + S::KV + stage * S::STAGE + kv_off<HD>(u / UPR, ch), tile + row[y] * g.row_bytes + ch * 16, unit, good);
             } else {
-              cp_async16_zfill(sb + S::RAW + (slot * UNITS + u) * 16, good ? tile + r * g.row_bytes + ch * 16 : tile, good);
+              cp_async16_zfill(sb + S::RAW + (slot * UNITS + u) * 16, tile + row[y] * g.row_bytes + ch * 16, unit, good);
+              const uint8_t* meta = tile + g.bs * g.row_bytes + row[y] * g.meta_row_bytes;
               const int q = (ch * EPU) >> a.gs_log2;
-              const uint8_t* meta = good ? tile + g.bs * g.row_bytes + r * g.meta_row_bytes + q * (a.mf32 ? 8 : 4) : g.base;
-              if (a.mf32) cp_async_zfill<8>(raw_meta + (slot * UNITS + u) * 8, meta, good);
-              else cp_async_zfill<4>(raw_meta + (slot * UNITS + u) * 4, meta, good);
+              if (a.mf32) cp_async_zfill<8>(raw_meta + (slot * UNITS + u) * 8, meta + q * 8, unit, good);
+              else cp_async_zfill<4>(raw_meta + (slot * UNITS + u) * 4, meta + q * 4, unit, good);
             }
           }
         };
@@ -1045,15 +1053,15 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           else convert_as(i, stage, slot, std::true_type(), std::false_type());
         };
         auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, abort_flag, err); };
-        int32_t ids[N];
-        fetch_ids(0, ids);
+        int32_t ids[N], rows[N];
+        fetch_ids(0, ids, rows);
         int in = 0, out = 0;  // ring slots of the next copy and the next conversion
         for (int i = 0; i < loads + depth - 1; ++i) {
           if (i < loads) {
             if (BITS == 0 && !empty(n + i)) break;
-            copy(i, ids, (n + i) % ST, in);
+            copy(i, ids, rows, (n + i) % ST, in);
             if (++in == depth) in = 0;
-            if (i + 1 < loads) fetch_ids(i + 1, ids);
+            if (i + 1 < loads) fetch_ids(i + 1, ids, rows);
           }
           cp_async_commit();
           const int d = i - (depth - 1);
@@ -1071,6 +1079,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           if (lane == 0) mbar_arrive(bar(BAR_FULL + (n + d) % ST));
         }
         n += loads;
+        if (bad) atomicOr(err, DEV_ERR_BLOCK);
       }
       if (!ok) break;
     }

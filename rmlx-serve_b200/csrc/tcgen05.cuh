@@ -69,13 +69,21 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// The same, or with live = false zeros and nothing read; N bytes, 4 or 8.
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+// The same if on; with live = false it writes zeros and reads nothing.  N bytes: 4 or 8.
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on, bool live) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(dst),
+      "l"(src), "r"(live ? 16 : 0), "r"((uint32_t)on)
+      : "memory");
 }
 template <int N>
-__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? N : 0), "n"(N) : "memory");
+__device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void* src, bool on, bool live) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "@p cp.async.ca.shared.global [%0], [%1], %4, %2;\n\t}" ::"r"(dst),
+      "l"(src), "r"(live ? N : 0), "r"((uint32_t)on), "n"(N)
+      : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
