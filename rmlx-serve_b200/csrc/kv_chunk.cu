@@ -123,6 +123,7 @@ constexpr int CH_HALF = 64;     // keys whose weights are made together
 // where they read and dequantise rows themselves.
 constexpr int ch_threads(bool tma) { return tma ? 384 : 512; }
 constexpr int CH_MAX_WARPS = 16;
+constexpr int CH_RAW = 4;       // most tiles of codes in flight
 constexpr int CH_OVERHEAD = 3;  // cost of an item besides its key tiles, in key tiles
 constexpr int CH_MIN_COST = 4;  // smallest share
 
@@ -272,7 +273,8 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // ---------------------------------------------------------------------------
 // The kernel.  S = Q K^T and O += P V on the tcgen05 tensor cores, S, P and O
 // in TMEM, K and V in a ring of shared-memory stages.  Warps 0-3 and 4-7 are
-// two softmax warpgroups (A and B), one thread a row; warp 8 issues the MMAs;
+// two softmax warpgroups (A and B), one thread a row (two a row, each with 64
+// of its columns, had to meet for the maximum: 8192-token prompt 654 us); warp 8 issues the MMAs;
 // warp 9 loads K and V tiles by TMA and warps 10-11 the queries (pools that
 // TMA cannot read: warps 9-15 load all).
 //   more than 128 rows: A and B hold rows 0-127 and 128-255 and every key tile
@@ -299,7 +301,8 @@ struct ChunkParams {
   PoolGeo g;
   ChunkArgs a;
   int tpt;                 // chunk tokens of a tile
-  int box;                 // rows of a TMA box
+  int box;                 // rows of a TMA box, or of a bulk copy of codes
+  int raw_depth;           // tiles of codes in flight by bulk copies, 0: codes are copied by the load warps
   float* parts;
   PartDesc* desc;
 };
@@ -309,18 +312,19 @@ struct ChunkSmem {
   static constexpr int QTILE = 128 * HD * 2;
   static constexpr int STAGE = CH_KEYS * HD * 2;
   // Quantised pools give two stages up for codes in flight (RAW): 3 tiles of
-  // 16-byte units of 8-bit codes with f16 scales, or 4 of 4-bit codes.
+  // 8-bit codes with f16 scales, or 4 of 4-bit codes.
   static constexpr int STAGES = BITS ? (HD == 128 ? 3 : 6) : HD == 128 ? 5 : 8;
   static constexpr int UNITS = BITS ? CH_KEYS * HD * BITS / 128 : 0;  // of a tile
   static constexpr int RAW_BYTES = BITS == 8 ? UNITS * 60 : UNITS * 96;
   static constexpr int Q = 0, KV = 2 * QTILE, RAW = KV + STAGES * STAGE, CTRL = RAW + RAW_BYTES;
   // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales
-  static constexpr int BARS = CTRL, PLAN = CTRL + 320, ML = PLAN + 128, QSCALE = ML + 1024;
+  static constexpr int BARS = CTRL, PLAN = CTRL + 352, ML = PLAN + 128, QSCALE = ML + 1024;
   static constexpr int BYTES = QSCALE + 512;
 };
 // barrier numbers
 constexpr int BAR_FULL = 0, BAR_EMPTY = 8, BAR_QFULL = 16, BAR_QEMPTY = 17, BAR_OFREE = 18, BAR_ML = 19, BAR_O = 20,
-              BAR_S = 22, BAR_V = 24, BAR_P = 26, BAR_DRAIN = 30;  // P: warpgroup * 2 + half
+              BAR_S = 22, BAR_V = 24, BAR_P = 26, BAR_DRAIN = 30, BAR_RAWF = 31,
+              BAR_RAWE = 35;  // P: warpgroup * 2 + half; RAW: up to CH_RAW slots
 
 template <int DT>
 __device__ __forceinline__ float unpack_lo(uint32_t w) {
@@ -493,15 +497,19 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
   constexpr uint32_t IDESC_S = mma_idesc(CT == RMLX_BF16, 128, CH_KEYS, false);
   constexpr uint32_t IDESC_O = mma_idesc(CT == RMLX_BF16, 128, HD, true);
   constexpr uint32_t TM_S = 0, TM_O = 256;  // TMEM columns: S/P of A and B, then O of A and B
-  constexpr int QWARPS = TMA ? 2 : 7;       // warps that load queries
+  // Load warps beside the one that issues TMA or bulk copies (none does where
+  // rows are copied by the load warps themselves): they load queries, and rows
+  // or codes.
+  const bool raw = BITS && p.raw_depth;
+  const int qwarps = TMA ? 2 : raw ? 6 : 7;
   extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms are 1024 bytes
   const uint32_t sb = smem_u32(smem);
   const PoolGeo& g = p.g;
   const ChunkArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto bar = [&](int i) { return sb + S::BARS + 8 * i; };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + 304);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 308);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + 336);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 340);
   ItemIter* plan = reinterpret_cast<ItemIter*>(smem + S::PLAN);
   float2* ml_b = reinterpret_cast<float2*>(smem + S::ML);
   uint8_t* qscale = smem + S::QSCALE;  // [2][CH_ROWS] f32 exponents, by item parity
@@ -509,10 +517,10 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < ST; ++i) {
-      mbar_init(bar(BAR_FULL + i), TMA ? 1 : QWARPS);
+      mbar_init(bar(BAR_FULL + i), TMA ? 1 : qwarps);
       mbar_init(bar(BAR_EMPTY + i), 1);
     }
-    mbar_init(bar(BAR_QFULL), QWARPS);
+    mbar_init(bar(BAR_QFULL), qwarps);
     mbar_init(bar(BAR_QEMPTY), 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(bar(BAR_S + x), 1);
@@ -522,11 +530,12 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       mbar_init(bar(BAR_P + 2 * x + 1), 4);
     }
     mbar_init(bar(BAR_DRAIN), 1);
+    for (int i = 0; i < CH_RAW; ++i) mbar_init(bar(BAR_RAWF + i), 1), mbar_init(bar(BAR_RAWE + i), 6);
     mbar_init(bar(BAR_OFREE), 8);
     mbar_init(bar(BAR_ML), 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tmem_alloc(sb + S::BARS + 308, 512);
+  if (warp == 8) tmem_alloc(sb + S::BARS + 340, 512);
   pdl_wait();
   pdl_release();
   PartDesc* desc = p.desc + 2 * blockIdx.x;
@@ -848,8 +857,9 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     // ---- loads ----------------------------------------------------------------
     uint32_t n = 0, nitem = 0;
     bool ok = true;
-    const bool loads_q = !TMA || warp >= 10, loads_kv = !TMA || warp == 9;
-    const int qw = TMA ? warp - 10 : warp - 9;
+    const bool issues = (TMA || raw) && warp == 9, loads_q = !issues;
+    const bool loads_kv = issues || !TMA;
+    const int qw = TMA || raw ? warp - 10 : warp - 9;
     for (bool more = next_portion(it, a, g.heads, p.tpt, true); more;
          more = next_portion(it, a, g.heads, p.tpt, false)) {
       const int nk = it.k1 - it.k0;
@@ -861,7 +871,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         constexpr int CPR = HD / 8, RPW = 32 / CPR;  // 16-byte chunks of a row, rows of a warp's pass
         const uint8_t* qbase = a.q + (int64_t)(it.qoff + it.t.t0) * a.qts + (int64_t)it.head * a.G * a.qhs;
         const int ch = lane % CPR;
-        const int step = QWARPS * RPW;
+        const int step = qwarps * RPW;
         if (!BITS) {
           // every row's copy in flight at once
           for (int r = qw * RPW + lane / CPR; r < it.t.rows; r += step) {
@@ -871,24 +881,22 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           }
           cp_async_wait_all();
         } else {
-        constexpr int U = 8;
-        for (int r0 = (qw * RPW) + lane / CPR; r0 < it.t.rows + (int)(lane / CPR); r0 += U * step) {
-          uint4 w[U];
+          constexpr int U = 8;
+          for (int r0 = (qw * RPW) + lane / CPR; r0 < it.t.rows + (int)(lane / CPR); r0 += U * step) {
+            uint4 w[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * step;
-            w[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < it.t.rows) {
-              const int tok = r / a.G;
-              w[u] = ld_stream(qbase + tok * a.qts + (r - tok * a.G) * a.qhs + ch * 16);
+            for (int u = 0; u < U; ++u) {
+              const int r = r0 + u * step;
+              w[u] = make_uint4(0u, 0u, 0u, 0u);
+              if (r < it.t.rows) {
+                const int tok = r / a.G;
+                w[u] = ld_stream(qbase + tok * a.qts + (r - tok * a.G) * a.qhs + ch * 16);
+              }
             }
-          }
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * step;
-            {
-              // the row's power of two, and a bf16 row in f16
-              int e = 127;
+            for (int u = 0; u < U; ++u) {
+              const int r = r0 + u * step;
+              int e = 127;  // the row's power of two, and a bf16 row in f16
               if (DT == RMLX_BF16) {
                 uint32_t* q4 = reinterpret_cast<uint32_t*>(&w[u]);
                 float mx = 0.0f;
@@ -904,11 +912,9 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
                 for (int i = 0; i < 4; ++i) q4[i] = pack2<RMLX_F16>(unpack_lo<DT>(q4[i]) * inv, unpack_hi<DT>(q4[i]) * inv);
               }
               if (ch == 0 && r < CH_ROWS) qscale[(nitem & 1) * CH_ROWS + r] = (uint8_t)e;
+              if (r < it.t.rows) sts128(sb + S::Q + (r >> 7) * S::QTILE + q_off<HD>(r & 127, ch), w[u]);
             }
-            if (r < it.t.rows)
-              sts128(sb + S::Q + (r >> 7) * S::QTILE + q_off<HD>(r & 127, ch), w[u]);
           }
-        }
         }
         fence_async_smem();
         __syncwarp();
@@ -952,6 +958,86 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
                             (t - b * g.bs) / 8,
                         bar(BAR_FULL + stage));
         }
+      } else if (raw) {
+        // Codes of a tile, then its (scale, zero) rows, as they lie in the blocks:
+        // warp 9 copies both a block's run at a time, the others convert them.
+        constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8, UPR = HD / EPU, UNITS = CH_KEYS * UPR, W = 6;
+        constexpr int N = (UNITS + 32 * W - 1) / (32 * W);
+        constexpr int RB = HD * BITS / 8;
+        const int mb = g.meta_row_bytes, depth = p.raw_depth;
+        const uint32_t raw_tile = CH_KEYS * (RB + mb);
+        const int64_t block_bytes = (int64_t)g.layers * 2 * g.heads * g.tile_bytes;
+        const uint8_t* head_base = g.base + g.tile_off(0, a.layer, 0, it.head);
+        for (int i = 0; i < loads; ++i) {
+          int j, kv;
+          which(i, j, kv);
+          const uint32_t slot = n % depth, phase = (n / depth) & 1, dst = sb + S::RAW + slot * raw_tile;
+          const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
+          if (warp == 9) {
+            if (!(ok = mbar_wait(bar(BAR_RAWE + slot), phase ^ 1, abort_flag, err))) break;
+            const int t = kb + lane * p.box;
+            const bool want = lane * p.box < CH_KEYS && t < it.t.hi;
+            int blk = 0, r = 0;
+            if (want) {
+              const int b = t / g.bs;
+              r = t - b * g.bs;
+              blk = __ldg(btrow + b);
+              if (blk < 0 || blk >= g.nblocks) {
+                atomicOr(err, DEV_ERR_BLOCK);
+                blk = 0;
+              }
+            }
+            const int boxes = __popc(__ballot_sync(0xffffffffu, want));
+            if (lane == 0) mbar_arrive_expect_tx(bar(BAR_RAWF + slot), boxes * p.box * (RB + mb));
+            __syncwarp();
+            if (want) {
+              const uint8_t* tile = head_base + blk * block_bytes + (kv ? (int64_t)g.heads * g.tile_bytes : 0);
+              bulk_load(dst + lane * p.box * RB, tile + r * RB, p.box * RB, bar(BAR_RAWF + slot));
+              bulk_load(dst + CH_KEYS * RB + lane * p.box * mb, tile + g.bs * RB + r * mb, p.box * mb, bar(BAR_RAWF + slot));
+            }
+          } else {
+            if (!(ok = mbar_wait(bar(BAR_RAWF + slot), phase, abort_flag, err))) break;
+            const uint32_t stage = n % ST, out = sb + S::KV + stage * S::STAGE;
+            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
+            const int ch = lane % UPR;
+            auto convert = [&](auto mf32, auto one) {  // f32 scales and zeros; a unit's elements are all of one group
+              constexpr bool MF32 = decltype(mf32)::value;
+#pragma unroll
+              for (int y = 0; y < N; ++y) {
+                const int u = (y * W + qw) * 32 + lane, row = u / UPR;
+                if (u >= UNITS) continue;
+                const uint4 w = lds128(dst + u * 16);
+                const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
+                const uint32_t meta = dst + CH_KEYS * RB + row * mb;
+                Group<BITS ? BITS : 8> grp;
+                auto group = [&](int e) {
+                  const int q = (ch * EPU + e) >> a.gs_log2;
+                  const uint2 sz = MF32 ? lds64(meta + q * 8) : make_uint2(lds32(meta + q * 4), 0u);
+                  grp.set(kb + row < it.t.hi ? sz : make_uint2(0u, 0u), MF32, kv);  // zeros behind the last visible row
+                };
+                group(0);
+                uint4 o[EPU / 8];
+#pragma unroll
+                for (int e = 0; e < EPU / 8; ++e) {
+                  if (!decltype(one)::value && e > 0) group(8 * e);
+                  o[e] = dequant8<BITS ? BITS : 8, MF32>(
+                      BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
+                }
+#pragma unroll
+                for (int e = 0; e < EPU / 8; ++e) sts128(out + kv_off<HD>(row, ch * (EPU / 8) + e), o[e]);
+              }
+            };
+            const bool one = (1 << a.gs_log2) >= EPU;
+            if (!a.mf32 && one) convert(std::false_type(), std::true_type());
+            else if (!a.mf32) convert(std::false_type(), std::false_type());
+            else if (one) convert(std::true_type(), std::true_type());
+            else convert(std::true_type(), std::false_type());
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(BAR_FULL + stage)), mbar_arrive(bar(BAR_RAWE + slot));
+          }
+          ++n;
+        }
       } else {
         // A unit is 16 bytes of a stored row: 8 elements, or 16 or 32 codes.  Rows
         // go straight into their stage; codes, with the scale and zero of a unit's
@@ -959,14 +1045,14 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         // copied them converts them `depth` - 1 loads later (with registers
         // instead of the ring one tile was in flight: 4-bit chunks 290 us).
         constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8, UPR = HD / EPU, UNITS = CH_KEYS * UPR;
-        constexpr int N = (UNITS + 32 * QWARPS - 1) / (32 * QWARPS);
+        constexpr int N = (UNITS + 32 * 7 - 1) / (32 * 7);
         const int depth = BITS == 0 ? 3 : BITS == 4 ? 4 : a.mf32 ? 2 : 3;
         const int ch = lane % UPR;  // the same for all of a lane's units
         const int64_t block_bytes = (int64_t)g.layers * 2 * g.heads * g.tile_bytes;
         const uint8_t* head_base = g.base + g.tile_off(0, a.layer, 0, it.head);
         const int u0 = qw * 32 + lane;
         const uint32_t raw_meta = sb + S::RAW + depth * UNITS * 16;
-        auto key_of = [&](int j, int y) { return (it.t.k_lo + it.k0 + j) * CH_KEYS + (u0 + y * QWARPS * 32) / UPR; };
+        auto key_of = [&](int j, int y) { return (it.t.k_lo + it.k0 + j) * CH_KEYS + (u0 + y * 7 * 32) / UPR; };
         // block ids (-1: no row) and rows in them of a load's units, a load ahead of the units themselves
         auto fetch_ids = [&](int i, int32_t (&blk)[N], int32_t (&row)[N]) {
           int j, kv;
@@ -982,7 +1068,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
           for (int y = 0; y < N; ++y) {
             blk[y] = -1;
-            if (u0 + y * QWARPS * 32 < UNITS && key_of(j, y) < it.t.hi) blk[y] = __ldg(btrow + b[y]);
+            if (u0 + y * 7 * 32 < UNITS && key_of(j, y) < it.t.hi) blk[y] = __ldg(btrow + b[y]);
           }
         };
         // straight-line, so that the units' address arithmetic overlaps
@@ -993,7 +1079,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           const uint8_t* base = head_base + (kv ? (int64_t)g.heads * g.tile_bytes : 0);
 #pragma unroll
           for (int y = 0; y < N; ++y) {
-            const int u = u0 + y * QWARPS * 32;
+            const int u = u0 + y * 7 * 32;
             const bool unit = u < UNITS, want = unit && key_of(j, y) < it.t.hi;
             const bool good = want && (uint32_t)blk[y] < (uint32_t)g.nblocks;  // else zeros
             bad |= want && !good;
@@ -1016,7 +1102,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           which(i, j, kv);
 #pragma unroll
           for (int y = 0; y < N; ++y) {
-            const int u = u0 + y * QWARPS * 32;
+            const int u = u0 + y * 7 * 32;
             if (u >= UNITS) continue;
             const uint4 w = lds128(sb + S::RAW + (slot * UNITS + u) * 16);
             const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
@@ -1083,10 +1169,12 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       }
       if (!ok) break;
     }
-    if (TMA && !ok && loads_kv)  // leave no copy in flight behind
-      for (uint32_t i = n > ST ? n - ST : 0; i < n; ++i)
-        for (int k = 0; k < (1 << 20) && !mbar_try(bar(BAR_FULL + i % ST), (i / ST) & 1); ++k) {
+    if (issues && !ok) {  // leave no copy in flight behind
+      const uint32_t slots = raw ? p.raw_depth : ST;
+      for (uint32_t i = n > slots ? n - slots : 0; i < n; ++i)
+        for (int k = 0; k < (1 << 20) && !mbar_try(bar((raw ? BAR_RAWF : BAR_FULL) + i % slots), (i / slots) & 1); ++k) {
         }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1172,6 +1260,11 @@ ChunkFn pick_chunk(int bits, bool tma) {
 template <int HD>
 size_t chunk_smem(int bits) {
   return bits == 8 ? ChunkSmem<HD, 8>::BYTES : bits == 4 ? ChunkSmem<HD, 4>::BYTES : ChunkSmem<HD, 0>::BYTES;
+}
+
+template <int HD>
+int chunk_raw(int bits) {
+  return bits == 8 ? ChunkSmem<HD, 8>::RAW_BYTES : ChunkSmem<HD, 4>::RAW_BYTES;
 }
 
 size_t chunk_workspace(const rmlx_kv_pool* p) {
@@ -1262,6 +1355,13 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   // TMA reads whole groups of 8 stored rows; a box is the most rows that both a block and a key tile hold a whole number of
   prm.box = std::gcd(c.block_size, CH_KEYS);
   const bool tma = !c.quant_bits && c.block_size % 8 == 0;
+  // codes and their (scale, zero) rows by bulk copies where a box of either is whole 16-byte pieces (and 32 lanes issue a tile's)
+  prm.raw_depth = 0;
+  if (c.quant_bits && prm.box >= 4 && prm.box * p->meta_row_bytes % 16 == 0) {
+    const int room = c.head_dim == 128 ? chunk_raw<128>(c.quant_bits) : chunk_raw<64>(c.quant_bits);
+    const int depth = std::min<int>(CH_RAW, room / (CH_KEYS * (int)(p->row_bytes + p->meta_row_bytes)));
+    if (depth >= 2) prm.raw_depth = depth;
+  }
   prm.parts = static_cast<float*>(workspace);
   prm.desc = reinterpret_cast<PartDesc*>(prm.parts + (size_t)p->num_sms * 2 * part_floats(c.head_dim));
   CUtensorMap map = {};
