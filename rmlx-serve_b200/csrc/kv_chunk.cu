@@ -1250,6 +1250,7 @@ using namespace rmlx;
 namespace {
 
 using ChunkFn = void (*)(ChunkParams, CUtensorMap, int32_t*);
+using ChunkCombineFn = void (*)(ChunkParams, int);
 template <int DT, int HD>
 ChunkFn pick_chunk(int bits, bool tma) {
   if (bits == 8) return chunk_attn_kernel<DT, HD, 8, false>;
@@ -1364,16 +1365,23 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   }
   prm.parts = static_cast<float*>(workspace);
   prm.desc = reinterpret_cast<PartDesc*>(prm.parts + (size_t)p->num_sms * 2 * part_floats(c.head_dim));
-  CUtensorMap map = {};
-  if (tma && (s = chunk_map(p, prm.box, &map)) != RMLX_OK) return s;
-  ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
-                                 : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
+  static_assert(sizeof(CUtensorMap) == sizeof(p->chunk_map), "tensor map");
   const size_t smem = c.head_dim == 128 ? chunk_smem<128>(c.quant_bits) : chunk_smem<64>(c.quant_bits);
-  if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
-  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(ch_threads(tma)), smem, (cudaStream_t)stream, prm, map, p->err);
+  if (!p->chunk_fn) {  // the first call of a pool
+    if (tma && (s = chunk_map(p, prm.box, reinterpret_cast<CUtensorMap*>(p->chunk_map))) != RMLX_OK) return s;
+    ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
+                                   : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
+    if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
+    p->chunk_fn = reinterpret_cast<void*>(fn);
+    p->chunk_combine_fn = reinterpret_cast<void*>(
+        c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
+                          : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>));
+  }
+  ChunkFn fn = reinterpret_cast<ChunkFn>(p->chunk_fn);
+  ChunkCombineFn fc = reinterpret_cast<ChunkCombineFn>(p->chunk_combine_fn);
+  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(ch_threads(tma)), smem, (cudaStream_t)stream, prm,
+                             *reinterpret_cast<const CUtensorMap*>(p->chunk_map), p->err);
   if (e != cudaSuccess) return cuda_check(e, "chunk attention launch");
-  auto fc = c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
-                              : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>);
   e = launch_pdl(fc, dim3(p->num_sms, CH_ROWS / 32), dim3(256), 0, (cudaStream_t)stream, prm, (int)p->num_sms);
   if (e != cudaSuccess) return cuda_check(e, "chunk attention combine launch");
   return cuda_check(cudaGetLastError(), "chunk attention launch");

@@ -107,6 +107,9 @@ struct rmlx_kv_pool {
   void* attn_fn = nullptr;
   size_t attn_smem = 0;
   int64_t attn_target = 0;
+  // The chunk attention's kernels (made ready once) and the pool as TMA sees it (a CUtensorMap).
+  void *chunk_fn = nullptr, *chunk_combine_fn = nullptr;
+  alignas(64) uint8_t chunk_map[128] = {};
   rmlx::PoolGeo geo() const {
     rmlx::PoolGeo g;
     g.base = base;

@@ -24,10 +24,19 @@ def _ptr(x) -> Optional[int]:
     return x.data_ptr()
 
 
+_raw_stream = None
+
+
 def _stream(stream, device: int) -> Optional[int]:
     if stream is None:
-        import torch
-        return torch.cuda.current_stream(device).cuda_stream
+        # torch's current stream as an address, without making a Stream object (a decode step's call is host-bound)
+        global _raw_stream
+        if _raw_stream is None:
+            import torch
+            torch.cuda.init()
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda d: torch.cuda.current_stream(d).cuda_stream)
+        return _raw_stream(device)
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
