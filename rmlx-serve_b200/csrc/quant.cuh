@@ -74,6 +74,29 @@ __device__ __forceinline__ uint32_t quant_code(float v, float mn, float scale, f
   return (x == x) ? (uint32_t)x : 0u;
 }
 
+// The codes of 8 elements: quant_code's, mostly without its division.  With x
+// = (v - mn) / scale <= 256 and inv = 1 / scale rounded, d * inv is within x
+// 2^-24 <= 2^-16 of x, and so is the rounded quotient that quant_code rounds.
+// Where d * inv lies more than 2^-13 from every tie, all three round to the
+// same code; elements nearer to one (1 in 4096), NaN, and scales whose
+// reciprocal loses digits take quant_code itself.
+__device__ __forceinline__ void quantise_codes(const float (&f)[8], float mn, float scale, float qmax, uint32_t (&code)[8]) {
+  const float inv = scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : __uint_as_float(0x7fffffffu);
+  bool sure = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float d = __fsub_rn(f[e], mn);
+    const float t = __fmaf_rn(d, inv, 12582912.0f);  // 1.5 * 2^23: the nearest integer in the low bits
+    const float off = __fmaf_rn(d, inv, 12582912.0f - t);
+    sure = sure && fabsf(off) <= 0.5f - 1.0f / 8192.0f;
+    code[e] = __float_as_uint(t) & 0xffu;
+  }
+  if (!sure) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) code[e] = quant_code(f[e], mn, scale, qmax);
+  }
+}
+
 // Quantises this lane's 8 elements f (chunk c of the row of KV head h) and
 // stores codes and, once per group, (scale, zero) in pool slot s of `layer`.
 // A group is tpg adjacent lanes, reduced with xor shuffles: every lane of
@@ -97,20 +120,15 @@ __device__ __forceinline__ void quantise8(const PoolGeo& g, const float (&f)[8],
   const int blk = s / g.bs, off = s - blk * g.bs;
   uint8_t* tile = g.base + g.tile_off(blk, layer, kv, h);
   uint8_t* code_row = tile + (int64_t)off * g.row_bytes;
+  uint32_t code[8];
+  quantise_codes(f, mn, scale, qmax, code);
   if (BITS == 8) {
-    uint32_t lo = 0, hi = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) lo |= quant_code(f[e], mn, scale, qmax) << (8 * e);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) hi |= quant_code(f[4 + e], mn, scale, qmax) << (8 * e);
-    *reinterpret_cast<uint2*>(code_row + c * 8) = make_uint2(lo, hi);
+    *reinterpret_cast<uint2*>(code_row + c * 8) =
+        make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
   } else {
     uint32_t w = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t a = quant_code(f[2 * e], mn, scale, qmax), b = quant_code(f[2 * e + 1], mn, scale, qmax);
-      w |= (a | (b << 4)) << (8 * e);
-    }
+    for (int e = 0; e < 8; ++e) w |= code[e] << (4 * e);
     *reinterpret_cast<uint32_t*>(code_row + c * 4) = w;
   }
   if ((c & (tpg - 1)) == 0) {
