@@ -414,18 +414,20 @@ __device__ __forceinline__ uint2 load_meta(const uint8_t* meta, int q, bool mf32
   return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(meta) + q), 0u);
 }
 // A group's scale and zero as the conversion takes them.  Its values lie
-// between zr and zr + qmax sc: where they leave f16's range, or where V's are
-// so small that f16 would lose their digits, the scale becomes NaN, and the
-// rows that see them take the exact path.
+// between zr and zr + qmax sc: where they leave f16's range, or where the
+// largest is below 2^-13, so that f16's smallest step (rounding 2^-25) would
+// cost more than 2^-12 of it, the scale becomes NaN, and the rows that see the
+// group take the exact path.
 template <int BITS>
 struct Group {
   float sc, zr;
   __half2 sc2, zr2;
-  __device__ __forceinline__ void set(uint2 meta, bool mf32, bool is_v) {
+  __device__ __forceinline__ void set(uint2 meta, bool mf32) {
     float s = mf32 ? __uint_as_float(meta.x) : unpack_lo<RMLX_F16>(meta.x);
     const float z = mf32 ? __uint_as_float(meta.y) : unpack_hi<RMLX_F16>(meta.x);
     const float top = fmaxf(fabsf(z), fabsf(fmaf((float)((1 << BITS) - 1), s, z)));
-    if (!(top <= 65504.0f) || (is_v && top > 0.0f && top < 3.0517578125e-5f)) s = __uint_as_float(0x7fffffffu);
+    const float least = s == 1.0f ? fabsf(z) : top;  // a flat group has scale 1 and no code but 0
+    if (!(top <= 65504.0f) || (least > 0.0f && least < 1.220703125e-4f)) s = __uint_as_float(0x7fffffffu);
     sc = s, zr = z;
     sc2 = __float2half2_rn(s), zr2 = __float2half2_rn(z);
   }
@@ -850,7 +852,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     }
     if (!ok) {  // leave no MMA in flight behind
       tc_commit(bar(BAR_DRAIN));
-      for (int i = 0; i < (1 << 20) && !mbar_try(bar(BAR_DRAIN), 0); ++i) {
+      for (int i = 0; i < 2000 && !mbar_try(bar(BAR_DRAIN), 0); ++i) {
       }
     }
   } else {
@@ -1013,7 +1015,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
                 auto group = [&](int e) {
                   const int q = (ch * EPU + e) >> a.gs_log2;
                   const uint2 sz = MF32 ? lds64(meta + q * 8) : make_uint2(lds32(meta + q * 4), 0u);
-                  grp.set(kb + row < it.t.hi ? sz : make_uint2(0u, 0u), MF32, kv);  // zeros behind the last visible row
+                  grp.set(kb + row < it.t.hi ? sz : make_uint2(0u, 0u), MF32);  // zeros behind the last visible row
                 };
                 group(0);
                 uint4 o[EPU / 8];
@@ -1108,7 +1110,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
             Group<BITS ? BITS : 8> grp;
             grp.set(MF32 ? lds64(raw_meta + (slot * UNITS + u) * 8) : make_uint2(lds32(raw_meta + (slot * UNITS + u) * 4), 0u),
-                    MF32, kv);
+                    MF32);
             const uint8_t* meta = nullptr;
             if (!decltype(one)::value) {
               const int t = key_of(j, y);
@@ -1122,7 +1124,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
             for (int e = 0; e < EPU / 8; ++e) {
               if (!decltype(one)::value && e > 0 && meta)
-                grp.set(load_meta(meta, (ch * EPU + 8 * e) >> a.gs_log2, MF32), MF32, kv);
+                grp.set(load_meta(meta, (ch * EPU + 8 * e) >> a.gs_log2, MF32), MF32);
               o[e] = dequant8<BITS ? BITS : 8, MF32>(
                   BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
             }
@@ -1172,7 +1174,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     if (issues && !ok) {  // leave no copy in flight behind
       const uint32_t slots = raw ? p.raw_depth : ST;
       for (uint32_t i = n > slots ? n - slots : 0; i < n; ++i)
-        for (int k = 0; k < (1 << 20) && !mbar_try(bar((raw ? BAR_RAWF : BAR_FULL) + i % slots), (i / slots) & 1); ++k) {
+        for (int k = 0; k < 2000 && !mbar_try(bar((raw ? BAR_RAWF : BAR_FULL) + i % slots), (i / slots) & 1); ++k) {
         }
     }
   }

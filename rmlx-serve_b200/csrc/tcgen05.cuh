@@ -20,11 +20,14 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// One try, which the hardware lets sleep for up to about a millisecond (with
+// its default, tens of thousands of tries a launch drew power from a kernel
+// that runs at the power limit: 8192-token prompt 2.5 % slower).
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000000;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
@@ -44,7 +47,7 @@ __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, vo
 #pragma unroll 1
   for (uint32_t i = 0; i < (1u << 28); ++i) {
     if (mbar_try(bar, parity)) return true;
-    if ((i & 255) == 255 && (*abort_flag || global_ns() - t0 > 4000000000ull)) break;
+    if ((i & 15) == 15 && (*abort_flag || global_ns() - t0 > 4000000000ull)) break;
   }
   *abort_flag = 1;
   atomicOr(err, DEV_ERR_TIMEOUT);
@@ -53,7 +56,7 @@ __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, vo
 // The wait of one thread.
 __device__ __forceinline__ bool mbar_wait_thread(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
 #pragma unroll 1
-  for (int i = 0; i < 64; ++i)
+  for (int i = 0; i < 16; ++i)
     if (mbar_try(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, abort_flag, err);
 }

@@ -107,7 +107,7 @@ def check(pool, layer, q, G, bt, q_lens, lens, window, out, dt):
             err = (got[skip:] - want).abs()
             assert torch.isfinite(got).all()
             rel = eps / 2 + 2.0 ** -10 + 2.0 ** -10 * reach + 2e-4 if c.quant_bits else eps + 2e-4
-            tol = rel * A + 2.0 ** -24
+            tol = rel * A + (2.0 ** -24 if dt == orc.F16 else 1e-38)
             assert (err <= tol).all(), (n, L, float((err / tol).max()))
         at += n
 
@@ -268,6 +268,28 @@ def test_masked_rows_quantised(cuda):
     assert torch.isfinite(outs[1][:5]).all()
     assert (outs[0][:5] - outs[1][:5]).abs().max() <= 2 * (2.0 ** -7 + 2e-4) * v.float().abs().max()
     assert torch.isnan(outs[1][5:]).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("kscale,vscale,qscale", [(1.0, 1e6, 1.0), (1e6, 1.0, 1e-6), (1e-6, 1e-7, 1e6), (30.0, 40.0, 1e-2), (1e-3, 1e-3, 1e20)])
+def test_value_ranges_of_quantised_pools(cuda, bits, kscale, vscale, qscale):
+    """bf16 rows far outside f16's range, and near its smallest values; the exact path takes the rows that see them."""
+    H, G, D, bs, dt = 2, 4, 128, 16, orc.BF16
+    g = torch.Generator("cuda").manual_seed(14)
+    pool = rmlx_kv.KVPool(1, H, D, bs, 20, dtype=dt, quant_bits=bits, group_size=32, meta_dtype=orc.F32)
+    if qscale > 1e10:  # scores of order 1 from keys of 1e-20
+        kscale = 1e-20
+    k, v = ((torch.randn(320, H, D, generator=g, device="cuda") * s).to(TORCH[dt]) for s in (kscale, vscale))
+    v[:200, :, :32] = 3e-6 * vscale  # groups of one value
+    v[200:, :, 64:96] = 0
+    pool.append(k, v, torch.arange(320, dtype=torch.int32, device="cuda"), 320)
+    q = (torch.randn(45, H * G, D, generator=g, device="cuda") * qscale).to(TORCH[dt])
+    out = torch.empty_like(q)
+    ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda")
+    bt = torch.arange(20, dtype=torch.int32, device="cuda")[None]
+    pool.chunk_attention(0, q, G, bt, 20, dev([45]), dev([310]), 1, 45, D ** -0.5, out, ws)
+    assert pool.check() == 0
+    check(pool, 0, q, G, bt, [45], [310], 0, out, dt)
 
 
 def test_large_scores(cuda):
