@@ -1004,24 +1004,31 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             const int ch = lane % UPR;
             auto convert = [&](auto mf32, auto one) {  // f32 scales and zeros; a unit's elements are all of one group
               constexpr bool MF32 = decltype(mf32)::value;
+              // every unit's loads first, so that the conversions overlap
+              auto unit = [&](int y) { return (y * W + qw) * 32 + lane; };
+              auto there = [&](int y) { return (y + 1) * W * 32 <= UNITS || unit(y) < UNITS; };
+              auto pair = [&](int y, int e) {
+                const uint32_t meta = dst + CH_KEYS * RB + unit(y) / UPR * mb;
+                const int q = (ch * EPU + e) >> a.gs_log2;
+                return MF32 ? lds64(meta + q * 8) : make_uint2(lds32(meta + q * 4), 0u);
+              };
+              uint4 ws[N];
+              uint2 sz[N];
+#pragma unroll
+              for (int y = 0; y < N; ++y)
+                if (there(y)) ws[y] = lds128(dst + unit(y) * 16), sz[y] = pair(y, 0);
 #pragma unroll
               for (int y = 0; y < N; ++y) {
-                const int u = (y * W + qw) * 32 + lane, row = u / UPR;
-                if (u >= UNITS) continue;
-                const uint4 w = lds128(dst + u * 16);
-                const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
-                const uint32_t meta = dst + CH_KEYS * RB + row * mb;
+                if (!there(y)) continue;
+                const int row = unit(y) / UPR;
+                const bool live = kb + row < it.t.hi;  // else zeros: behind the last visible row
+                const uint32_t cw[4] = {ws[y].x, ws[y].y, ws[y].z, ws[y].w};
                 Group<BITS ? BITS : 8> grp;
-                auto group = [&](int e) {
-                  const int q = (ch * EPU + e) >> a.gs_log2;
-                  const uint2 sz = MF32 ? lds64(meta + q * 8) : make_uint2(lds32(meta + q * 4), 0u);
-                  grp.set(kb + row < it.t.hi ? sz : make_uint2(0u, 0u), MF32);  // zeros behind the last visible row
-                };
-                group(0);
+                grp.set(live ? sz[y] : make_uint2(0u, 0u), MF32);
                 uint4 o[EPU / 8];
 #pragma unroll
                 for (int e = 0; e < EPU / 8; ++e) {
-                  if (!decltype(one)::value && e > 0) group(8 * e);
+                  if (!decltype(one)::value && e > 0) grp.set(live ? pair(y, 8 * e) : make_uint2(0u, 0u), MF32);
                   o[e] = dequant8<BITS ? BITS : 8, MF32>(
                       BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
                 }
