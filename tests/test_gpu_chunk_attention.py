@@ -245,6 +245,28 @@ def test_masked_rows_have_no_influence(cuda, junk, bs, D):
         assert torch.isnan(dirty[3:6]).all() and torch.isnan(dirty[26:46]).all()  # rows that do see it
 
 
+def test_every_row_through_the_exact_path(cuda):
+    """V holds an infinity that all tokens but the first few see: NaN or infinity there, the others exact."""
+    H, G, D, bs, dt = 1, 4, 64, 16, orc.BF16
+    g = torch.Generator("cuda").manual_seed(16)
+    pool = rmlx_kv.KVPool(1, H, D, bs, 320, dtype=dt)
+    fill(pool, dt, 0, g)
+    rows = pool_rows(pool, dt)
+    bt = torch.arange(320, dtype=torch.int32, device="cuda")[None]
+    at = 4930
+    q = torch.randn(200, G, D, generator=g, device="cuda").to(TORCH[dt])
+    ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda")
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    pool.chunk_attention(0, q, G, bt, 320, dev([200]), dev([5120]), 1, 200, D ** -0.5, clean, ws)
+    rows[at // bs, 0, 1, 0, at % bs] = float("inf")
+    pool.chunk_attention(0, q, G, bt, 320, dev([200]), dev([5120]), 1, 200, D ** -0.5, out, ws)
+    assert pool.check() == 0
+    first = at - 4920  # tokens before the infinity
+    assert torch.isfinite(out[:first]).all()
+    assert (out[:first].float() - clean[:first].float()).abs().max() <= 2 * (2.0 ** -7 + 2e-4) * 5.5
+    assert (out[first:] == float("inf")).all()
+
+
 def test_masked_rows_quantised(cuda):
     """Junk scales and zeros behind the end of a sequence and in later tokens of a quantised pool."""
     H, G, D, bs, dt = 1, 4, 128, 16, orc.BF16
