@@ -177,86 +177,104 @@ __device__ __forceinline__ bool next_portion(ItemIter& it, const ChunkArgs& a, i
   return true;
 }
 
-// Sum of x over the CTA's earlier threads; *total over all.  words: CH_MAX_WARPS 64-bit words of shared memory.
-__device__ __forceinline__ int64_t block_prefix(int64_t x, int64_t* words, int64_t* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t y = x;
+// Sums of x[i] over the CTA's earlier threads into x[i], over all into total[i].
+// words: N CH_MAX_WARPS 64-bit words of shared memory, read by nobody else before the next barrier.
+template <int N>
+__device__ __forceinline__ void block_prefix(int64_t (&x)[N], int64_t (&total)[N], int64_t* words) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int64_t y[N];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
-    if (lane >= o) y += z;
+  for (int i = 0; i < N; ++i) {
+    y[i] = x[i];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t z = __shfl_up_sync(0xffffffffu, y[i], o);
+      if (lane >= o) y[i] += z;
+    }
+    if (lane == 31) words[i * CH_MAX_WARPS + warp] = y[i];
   }
   __syncthreads();
-  if (lane == 31) words[warp] = y;
-  __syncthreads();
-  int64_t before = y - x, all = 0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-    if (w < warp) before += words[w];
-    all += words[w];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    // every warp scans the warps' sums, one a lane
+    int64_t w = lane < warps ? words[i * CH_MAX_WARPS + lane] : 0;
+    const int64_t own = __shfl_sync(0xffffffffu, w, warp);
+#pragma unroll
+    for (int o = 1; o < CH_MAX_WARPS; o <<= 1) {
+      const int64_t z = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += z;
+    }
+    total[i] = __shfl_sync(0xffffffffu, w, CH_MAX_WARPS - 1);
+    x[i] = y[i] - x[i] + __shfl_sync(0xffffffffu, w, warp) - own;
   }
-  *total = all;
-  return before;
+}
+
+// n / d with 32 bits where they do (a 64-bit division takes some hundred clocks).
+__device__ __forceinline__ int64_t div_small(int64_t n, int64_t d) {
+  if (((n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
+  return n / d;
 }
 
 // Cuts the work and leaves this CTA's share in *out (left = 0: none).
-// scratch: CH_MAX_WARPS 64-bit words, 2 (nseq + 1) words.  False when q_lens sum past
+// scratch: 3 CH_MAX_WARPS 64-bit words, 2 (nseq + 1) words.  False when q_lens sum past
 // a.nq.  Each thread walks a run of sequences, then a run of tiles.
 __device__ __forceinline__ bool make_plan(const ChunkArgs& a, int heads, int tpt, uint8_t* scratch, ItemIter* out,
                                           int32_t* err) {
   int64_t* words = reinterpret_cast<int64_t*>(scratch);
-  int32_t* cub = reinterpret_cast<int32_t*>(words + CH_MAX_WARPS);  // tiles before a sequence
-  int32_t* cut = cub + a.nseq + 1;                                     // chunk tokens before it
+  int32_t* cub = reinterpret_cast<int32_t*>(words + 3 * CH_MAX_WARPS);  // tiles before a sequence
+  int32_t* cut = cub + a.nseq + 1;                                      // chunk tokens before it
   const int tid = threadIdx.x;
   if (tid == 0) out->left = 0;
-  const int nt = blockDim.x, per_s = (a.nseq + nt - 1) / nt;
+  const int nt = blockDim.x, per_s = a.nseq <= nt ? 1 : (a.nseq + nt - 1) / nt;
   const int s0 = min(a.nseq, tid * per_s), s1 = min(a.nseq, s0 + per_s);
-  int64_t tokens = 0, tiles = 0, total;
+  int64_t before[2] = {0, 0}, all[2];  // tokens, tiles
   for (int s = s0; s < s1; ++s) {
-    const int q = max(__ldg(a.q_lens + s), 0);
-    tokens += q;
-    tiles += ((int64_t)q + tpt - 1) / tpt;
-    if (q > 0 && __ldg(a.seq_lens + s) > a.max_len && blockIdx.x == 0) atomicOr(err, DEV_ERR_BLOCK);
+    const int q = max(__ldg(a.q_lens + s), 0), len = __ldg(a.seq_lens + s);
+    before[0] += q;
+    before[1] += q ? (q - 1) / tpt + 1 : 0;
+    if (q > 0 && len > a.max_len && blockIdx.x == 0) atomicOr(err, DEV_ERR_BLOCK);
   }
-  int64_t before = block_prefix(tokens, words, &total);
-  if (total > a.nq) return false;
-  int64_t tile = block_prefix(tiles, words, &total);
+  block_prefix(before, all, words);
+  if (all[0] > a.nq) return false;
+  int token = (int)before[0], tile = (int)before[1];
   for (int s = s0; s < s1; ++s) {
-    cub[s] = (int32_t)tile, cut[s] = (int32_t)before;
+    cub[s] = tile, cut[s] = token;
     const int q = max(__ldg(a.q_lens + s), 0);
-    before += q;
-    tile += (q + tpt - 1) / tpt;
+    token += q;
+    tile += q ? (q - 1) / tpt + 1 : 0;
   }
-  if (s0 < s1 && s1 == a.nseq) cub[a.nseq] = (int32_t)tile, cut[a.nseq] = (int32_t)before;
+  if (tid == 0) cub[a.nseq] = (int)all[1], cut[a.nseq] = (int)all[0];
   __syncthreads();
-  const int T = cub[a.nseq], per = (T + nt - 1) / nt;
+  const int T = (int)all[1], per = T <= nt ? 1 : (T + nt - 1) / nt;
   const int beg = (int)min((int64_t)T, (int64_t)tid * per), end = min(T, beg + per);
-  auto walk = [&](auto&& f) {  // f(sequence, its chunk length, its rows, tile, tile's cost over all heads)
+  auto walk = [&](auto&& f) {  // f(sequence, its chunk length, its rows, tile, an item's cost)
     if (beg >= end) return;
     int s = find_seq(cub, a.nseq, beg);
     for (int i = beg; i < end; ++s) {
       const int qlen = cut[s + 1] - cut[s], len = min(max(__ldg(a.seq_lens + s), 0), a.max_len);
       for (const int stop = min(end, cub[s + 1]); i < stop; ++i) {
         const int mt = i - cub[s];
-        f(s, qlen, len, mt, (int64_t)heads * (tile_geo(qlen, len, mt, tpt, a.G, a.window).nk + CH_OVERHEAD));
+        f(s, qlen, len, mt, tile_geo(qlen, len, mt, tpt, a.G, a.window).nk + CH_OVERHEAD);
       }
     }
   };
-  int64_t mine = 0;
-  walk([&](int, int, int, int, int64_t c) { mine += c; });
-  before = block_prefix(mine, words, &total);
-  const int64_t n = max((int64_t)1, min((int64_t)gridDim.x, total / CH_MIN_COST));
+  int64_t cost[1] = {0}, total[1];
+  walk([&](int, int, int, int, int one) { cost[0] += (int64_t)heads * one; });
+  const int64_t mine = cost[0];
+  block_prefix(cost, total, words + 2 * CH_MAX_WARPS);
+  const int64_t n = total[0] >= (int64_t)gridDim.x * CH_MIN_COST ? gridDim.x : max((int)total[0] / CH_MIN_COST, 1);
   if (blockIdx.x >= n) return true;
-  const int64_t b0 = total * blockIdx.x / n, b1 = total * (blockIdx.x + 1) / n;
-  if (b0 < b1 && before <= b0 && b0 < before + mine) {
-    int64_t c0 = before;
-    walk([&](int s, int qlen, int len, int mt, int64_t c) {
-      if (c0 <= b0 && b0 < c0 + c) {
-        const int64_t one = c / heads;
+  const int64_t b0 = div_small(total[0] * blockIdx.x, n), b1 = div_small(total[0] * (blockIdx.x + 1), n);
+  if (b0 < b1 && cost[0] <= b0 && b0 < cost[0] + mine) {
+    int64_t c0 = cost[0];
+    walk([&](int s, int qlen, int len, int mt, int one) {
+      if (c0 <= b0 && b0 < c0 + (int64_t)heads * one) {
+        const int head = (int)div_small(b0 - c0, one);
         out->s = s, out->mt = mt, out->qoff = cut[s], out->qlen = qlen, out->len = len;
-        out->head = (int)((b0 - c0) / one), out->off = (b0 - c0) % one;
+        out->head = head, out->off = b0 - c0 - (int64_t)head * one;
         out->left = b1 - b0;
       }
-      c0 += c;
+      c0 += (int64_t)heads * one;
     });
   }
   return true;
