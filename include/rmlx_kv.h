@@ -427,12 +427,14 @@ RMLX_API rmlx_status rmlx_kv_decode_attention(rmlx_kv_pool* p, int32_t layer, co
  * q: rows of all chunks back to back, num_q_tokens of them at least; row
  * (token, query head) at element token * q_token_stride + head *
  * q_head_stride.  out: [token][num_kv_heads * q_heads_per_kv][head_dim] in the
- * pool's type; rows behind the last chunk are left as they were.  When q_lens
+ * pool's type, not overlapping q; rows behind the last chunk are left as they
+ * were.  Lengths and tables are read on the device when the launch runs, so a
+ * captured launch follows them.  When q_lens
  * sum to more than num_q_tokens the launch is flagged (rmlx_kv_pool_check bit
  * 16) and writes nothing.  Block ids outside the pool, and a sequence of more
  * rows than block_table_stride blocks (or 2^30) hold, are flagged (bit 2); what
  * that sequence's out rows then hold is unspecified.  Waits inside the kernel
- * are bounded: one that runs out (seconds) is flagged (bit 32).
+ * are bounded: one that runs out (about 30 s) is flagged (bit 32).
  * Pools, head_dim and q_heads_per_kv as for rmlx_kv_decode_attention; any
  * block size.  A quantised pool's rows count as code * scale + zero, without
  * the gather's rounding to cfg.dtype.  workspace: rmlx_kv_chunk_attention_workspace_size bytes, not

@@ -74,13 +74,12 @@ __device__ __forceinline__ void load_row(const PoolGeo& g, const ChunkArgs& a, c
 // mask hides are never read.
 template <int DT, int HD>
 __device__ __forceinline__ void attend_row(const PoolGeo& g, const ChunkArgs& a, const int32_t* btrow, int h, int k0,
-                                           int k1, const float (&qf)[HD / 32], int lane, WaitState* ws, int32_t* err,
-                                           float& m, float& l, float (&acc)[HD / 32]) {
+                                           int k1, const float (&qf)[HD / 32], int lane, int32_t* err, float& m,
+                                           float& l, float (&acc)[HD / 32]) {
   constexpr int EPL = HD / 32;
   constexpr unsigned FULL = 0xffffffffu;
   const int64_t vdelta = (int64_t)g.heads * g.tile_bytes;
   for (int j = k0; j < k1; ++j) {
-    if (lane == 0 && (j & 4095) == 0) ++ws->beat;  // the CTA's other warps wait meanwhile
     const int b = j / g.bs;
     const int32_t blk = __ldg(btrow + b);
     if (blk < 0 || blk >= g.nblocks) {
@@ -305,7 +304,7 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // scores.  O is rescaled only when a row's maximum has grown by more than 2^8
 // since the last time (weights stay below 2^8; the final division undoes it).
 // Measured for an 8192-token prompt (8 x 128, G = 4, bf16): 573 us, 960 TFLOP/s
-// of the causal work, in short bursts; 631 us at the power limit.  A key tile
+// of the causal work, in short bursts; 623 us at the power limit.  A key tile
 // takes a warpgroup about 2460 clocks of softmax and 1750 of waiting for the two
 // products, the tensor cores 2060.  Slower were: two threads a row (654 us), an
 // MMA warp for each warpgroup (726), weights through shared memory so that the
@@ -538,14 +537,14 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
   const ChunkArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto bar = [&](int i) { return sb + S::BARS + 8 * i; };
-  WaitState* ws = reinterpret_cast<WaitState*>(smem + S::BARS + 336);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 344);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + 336);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BARS + 340);
   ItemIter* plan = reinterpret_cast<ItemIter*>(smem + S::PLAN);
   float2* ml_b = reinterpret_cast<float2*>(smem + S::ML);
   uint8_t* qscale = smem + S::QSCALE;  // [2][CH_ROWS] f32 exponents, by item parity
 
   if (threadIdx.x == 0) {
-    ws->failed = 0, ws->beat = 0;
+    *abort_flag = 0;
     for (int i = 0; i < ST; ++i) {
       mbar_init(bar(BAR_FULL + i), TMA ? 1 : qwarps);
       mbar_init(bar(BAR_EMPTY + i), 1);
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     mbar_init(bar(BAR_ML), 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tmem_alloc(sb + S::BARS + 344, 512);
+  if (warp == 8) tmem_alloc(sb + S::BARS + 340, 512);
   pdl_wait();
   pdl_release();
   PartDesc* desc = p.desc + 2 * blockIdx.x;
@@ -613,7 +612,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       bool ok = true;
       for (int j = 0; j < mine; ++j) {
         const int b = j & 1;
-        if (b == 0 && !(ok = mbar_wait(bar(BAR_S + x), ns++ & 1, ws, err))) break;
+        if (b == 0 && !(ok = mbar_wait(bar(BAR_S + x), ns++ & 1, abort_flag, err))) break;
         if (active) {
           tc_fence_after();
           if (BITS && j == 0) c = a.scale_log2 * __uint_as_float((uint32_t)qscale[(nitem & 1) * CH_ROWS + row] << 23);
@@ -647,7 +646,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             if (j > 0) {
               // products into O have to be done: those of earlier tiles are (these scores were issued
               // behind them), the tile's first half signals its own
-              if (b && !(ok = mbar_wait(bar(BAR_V + x), (ns - 1) & 1, ws, err))) break;
+              if (b && !(ok = mbar_wait(bar(BAR_V + x), (ns - 1) & 1, abort_flag, err))) break;
               tc_fence_after();
 #pragma unroll 1
               for (int i = 0; i < HD; i += 16) {
@@ -684,13 +683,13 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       const bool has[2] = {true, two || nk > 1};  // A and B have tiles
       if (!two) {
         if (x == 1) {
-          if (nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, ws, err))) break;
+          if (nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, abort_flag, err))) break;
           ml_b[wq * 32 + lane] = make_float2(ml, l);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(BAR_ML));
           writes = false;
         } else {
-          if (!(ok = mbar_wait(bar(BAR_ML), nml & 1, ws, err))) break;
+          if (!(ok = mbar_wait(bar(BAR_ML), nml & 1, abort_flag, err))) break;
           const float2 b = ml_b[wq * 32 + lane];
           const float n = fmaxf(ml, b.x);
           const float base = n == -INFINITY ? 0.0f : n;
@@ -704,7 +703,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
       for (int y = 0; y < 2 && ok; ++y) {
         // a warpgroup reads its own O, and A reads B's too when they share rows
-        if (has[y] && (y == x || (!two && x == 0))) ok = mbar_wait(bar(BAR_O + y), no[y] & 1, ws, err);
+        if (has[y] && (y == x || (!two && x == 0))) ok = mbar_wait(bar(BAR_O + y), no[y] & 1, abort_flag, err);
         no[y] += has[y];
       }
       if (!ok) break;
@@ -764,7 +763,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           for (int e = 0; e < EPL; ++e) qf[e] = unpack_lo<DT>(__ldg(qp + e)), acc[e] = 0.0f;
           const int k_first = (it.t.k_lo + it.k0) * CH_KEYS, k_end = (it.t.k_lo + it.k1) * CH_KEYS;
           attend_row<DT, HD>(g, a, a.bt + (int64_t)it.s * a.bt_stride, it.head, max(blow, k_first), min(blim, k_end),
-                             qf, lane, ws, err, bm, bl, acc);
+                             qf, lane, err, bm, bl, acc);
           const float bi = whole ? (bl == 0.0f ? 0.0f : 1.0f / bl) : 1.0f;
 #pragma unroll
           for (int e = 0; e < EPL; ++e) {
@@ -786,7 +785,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     uint32_t nitem = 0, pp = 0;  // items; a phase bit for each P buffer
     uint32_t st = 0, ph = 0;     // the ring's next stage and its phase
     bool ok = true;
-    auto wait = [&](int b, uint32_t parity) { return ok = ok && mbar_wait(bar(b), parity & 1, ws, err); };
+    auto wait = [&](int b, uint32_t parity) { return ok = ok && mbar_wait(bar(b), parity & 1, abort_flag, err); };
     auto advance = [&] {
       if (++st == ST) st = 0, ph ^= 1;
     };
@@ -897,7 +896,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       const bool two = it.t.rows > 128;
       const int32_t* btrow = a.bt + (int64_t)it.s * a.bt_stride;
       if (loads_q) {
-        if (nitem > 0 && !(ok = mbar_wait(bar(BAR_QEMPTY), (nitem - 1) & 1, ws, err))) break;
+        if (nitem > 0 && !(ok = mbar_wait(bar(BAR_QEMPTY), (nitem - 1) & 1, abort_flag, err))) break;
         constexpr int CPR = HD / 8, RPW = 32 / CPR;  // 16-byte chunks of a row, rows of a warp's pass
         const uint8_t* qbase = a.q + (int64_t)(it.qoff + it.t.t0) * a.qts + (int64_t)it.head * a.G * a.qhs;
         const int ch = lane % CPR;
@@ -965,7 +964,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           int j, kv;
           which(i, j, kv);
           const uint32_t stage = n % ST, dst = sb + S::KV + stage * S::STAGE;
-          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, ws, err))) break;
+          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
           ++n;
           // one box of p.box rows a lane
           const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS, t = kb + lane * p.box;
@@ -1004,7 +1003,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           const uint32_t slot = n % depth, phase = (n / depth) & 1, dst = sb + S::RAW + slot * raw_tile;
           const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
           if (warp == 9) {
-            if (!(ok = mbar_wait(bar(BAR_RAWE + slot), phase ^ 1, ws, err))) break;
+            if (!(ok = mbar_wait(bar(BAR_RAWE + slot), phase ^ 1, abort_flag, err))) break;
             const int t = kb + lane * p.box;
             const bool want = lane * p.box < CH_KEYS && t < it.t.hi;
             int blk = 0, r = 0;
@@ -1026,9 +1025,9 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
               bulk_load(dst + CH_KEYS * RB + lane * p.box * mb, tile + g.bs * RB + r * mb, p.box * mb, bar(BAR_RAWF + slot));
             }
           } else {
-            if (!(ok = mbar_wait(bar(BAR_RAWF + slot), phase, ws, err))) break;
+            if (!(ok = mbar_wait(bar(BAR_RAWF + slot), phase, abort_flag, err))) break;
             const uint32_t stage = n % ST, out = sb + S::KV + stage * S::STAGE;
-            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, ws, err))) break;
+            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
             const int ch = lane % UPR;
             auto convert = [&](auto mf32, auto one) {  // f32 scales and zeros; a unit's elements are all of one group
               constexpr bool MF32 = decltype(mf32)::value;
@@ -1175,7 +1174,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           else if (one) convert_as(i, stage, slot, std::true_type(), std::true_type());
           else convert_as(i, stage, slot, std::true_type(), std::false_type());
         };
-        auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, ws, err); };
+        auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, abort_flag, err); };
         int32_t ids[N], rows[N];
         fetch_ids(0, ids, rows);
         int in = 0, out = 0;  // ring slots of the next copy and the next conversion

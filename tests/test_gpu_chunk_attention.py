@@ -408,6 +408,36 @@ def test_prefill_in_chunks_with_prefix_reuse(cuda):
     assert pool.check() == 0
 
 
+def test_a_graph_follows_its_lengths(cuda):
+    """A captured call replayed after its lengths, tables and queries changed on the device; then with no chunk at all."""
+    H, G, D, bs, dt = 2, 4, 128, 16, orc.BF16
+    g = torch.Generator("cuda").manual_seed(17)
+    pool = rmlx_kv.KVPool(1, H, D, bs, 400, dtype=dt)
+    fill(pool, dt, 0, g)
+    width, T = 150, 400
+    bt = torch.zeros(3, width, dtype=torch.int32, device="cuda")
+    q_lens, lens = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(T, H * G, D, dtype=TORCH[dt], device="cuda")
+    out = torch.zeros_like(q)
+    ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pool.chunk_attention(0, q, G, bt, width, q_lens, lens, 3, T, D ** -0.5, out, ws)
+    for n, L in (([1, 1, 1], [5, 900, 2300]), ([300, 0, 90], [310, 70, 2000]), ([7, 200, 64], [2400, 200, 64]), ([0, 0, 0], [9, 9, 9])):
+        new = tables(L, bs, 400, g)
+        bt.zero_()
+        bt[:, :new.shape[1]] = new
+        q_lens.copy_(dev(n))
+        lens.copy_(dev(L))
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        out.fill_(4.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert pool.check() == 0
+        assert (out[sum(n):] == 4.0).all()
+        check(pool, 0, q, G, bt, n, L, 0, out, dt)
+
+
 def test_graphs_streams_and_bad_arguments(cuda):
     H, G, D, bs, dt = 2, 4, 64, 16, orc.BF16
     g = torch.Generator("cuda").manual_seed(12)
