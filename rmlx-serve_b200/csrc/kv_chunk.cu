@@ -126,6 +126,13 @@ constexpr int CH_MAX_WARPS = 16;
 constexpr int CH_RAW = 4;       // most tiles of codes in flight
 constexpr int CH_OVERHEAD = 3;  // cost of an item besides its key tiles, in key tiles
 constexpr int CH_MIN_COST = 4;  // smallest share
+// Weights are made as 2^(score - running maximum + bias).  A lagging maximum lets
+// them grow to 2^(8 + bias), which f16 holds up to a bias of 7; below 2^-14 f16
+// loses digits and below 2^-25 everything, so that without the bias the tail behind
+// one key of nearly all the weight came out short (16 nats behind it 6 %, 17.5
+// nats all).  bf16 has f32's range.
+template <int CT>
+constexpr float CH_BIAS = CT == RMLX_F16 ? 7.0f : 0.0f;
 
 // Chunk token range, key tiles and masks of tile mt of a sequence.
 struct TileGeo {
@@ -302,7 +309,8 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // warpgroup takes its 128 scores in halves: the first half's product runs while
 // the second half's weights are computed.  P overwrites the first half of its
 // scores.  O is rescaled only when a row's maximum has grown by more than 2^8
-// since the last time (weights stay below 2^8; the final division undoes it).
+// since the last time (weights stay below 2^8, times the bias of f16; the final
+// division undoes both).
 // Measured for an 8192-token prompt (8 x 128, G = 4, bf16): 573 us, 960 TFLOP/s
 // of the causal work, in short bursts; 623 us at the power limit.  A key tile
 // takes a warpgroup about 2460 clocks of softmax and 1750 of waiting for the two
@@ -660,7 +668,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
               tc_wait_st();
             }
           }
-          const float nb = m == -INFINITY ? 0.0f : -m * c;
+          const float nb = m == -INFINITY ? 0.0f : CH_BIAS<CT> - m * c;
           l += weights<CT>(v, c, nb, tm_s + CH_HALF * b);
           tc_wait_st();
           tc_fence_before();
@@ -670,7 +678,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       }
       if (!ok) break;
       // ---- epilogue ---------------------------------------------------------
-      float ml = m == -INFINITY ? -INFINITY : m * c;  // in the log2 domain
+      float ml = m == -INFINITY ? -INFINITY : m * c - CH_BIAS<CT>;  // in the log2 domain: O and l are in units of 2^ml
       const bool whole = it.k0 == 0 && it.k1 == it.t.nk;
       const int slot = it.k0 == 0 ? 1 : 0;
       float* part = p.parts + (size_t)(2 * blockIdx.x + slot) * part_floats(HD);

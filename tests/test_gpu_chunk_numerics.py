@@ -1,0 +1,100 @@
+"""Chunk attention (rmlx_kv_chunk_attention) where a value's range, not its formula, makes it hard.
+
+Bound of an element, with A = sum_j p_j |v_j| (p the softmax) and S = sum_j |v_j| over the row's visible keys:
+  * f16 products (f16 pools and all quantised ones): a weight is held relative to a running maximum m that is at most
+    the row's maximum and is scaled by 2^7, so it is rounded by half a step of f16, 2^-11 of it, or, below f16's
+    normal numbers, by at most 2^-25 2^-7 of the largest weight, which the sum of weights is never below:
+    |error| <= 2^-11 A + 2^-32 S.  bf16 products have f32's range: 2^-8 A (half a step of bf16 is 2^-9).
+  * the output's rounding: eps / 2 of |out| <= A, and half a step among the subnormals of f16 (2^-25);
+  * f32 scores, exponentials and sums: 2e-4 of A (as derived in test_gpu_chunk_attention.py), for scores of at most
+    64: a larger score s adds its own rounding, 2^-23 s, to each weight;
+  * quantised pools: a stored value code * scale + zero is rounded to f16 (2^-11 of it): 2^-11 A for V, and a score
+    off by delta <= 2^-11 scale sum |q_d k_d| for K, which moves weights and their sum by exp(2 delta) together.
+    Below f16's normal numbers the rounding is 2^-25: in f16 pools that is half a step of the output's own; in bf16
+    ones it stands only where the largest output of the element's group is 2^-13 or more, so 2^-12 of that largest.
+"""
+import numpy as np
+import pytest
+import torch
+
+import oracle as orc
+import rmlx_kv
+from test_gpu_append_rope import TORCH, pool_rows
+from test_gpu_chunk_attention import dev, stored_rows, tables
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(pool, q, G, bt, q_lens, lens, out=None, ws=None, window=0, scale=None):
+    """One call over contiguous q rows; the result."""
+    out = torch.empty_like(q) if out is None else out
+    ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda") if ws is None else ws
+    pool.chunk_attention(0, q, G, bt, bt.shape[1], dev(q_lens), dev(lens), len(lens), q.shape[0],
+                         pool.cfg.head_dim ** -0.5 if scale is None else scale, out, ws, window=window)
+    return out
+
+
+def check_rows(pool, q, G, bt, q_lens, lens, out, dt, window=0):
+    """Every out row against float64 over the stored rows, within the bound above."""
+    c = pool.cfg
+    H, D, bs = c.num_kv_heads, c.head_dim, c.block_size
+    rows = stored_rows(pool, 0, dt)
+    eps = torch.finfo(TORCH[dt]).eps
+    f16 = bool(c.quant_bits) or dt == orc.F16
+    at = 0
+    for s, (n, L) in enumerate(zip(q_lens, lens)):
+        blocks = bt[s, :-(-L // bs)].long().clamp(0, c.num_blocks - 1)  # a table may name no block below the window
+        kv = rows[blocks]
+        k, v = (kv[:, i].transpose(0, 1).reshape(H, -1, D)[:, :L] for i in (0, 1))
+        pos = torch.arange(L - n, L, device="cuda")[:, None]
+        key = torch.arange(L, device="cuda")[None]
+        seen = (key <= pos) & ((key > pos - window) if window else True)
+        used = seen.any(0)
+        k, v = (torch.where(used[None, :, None], x, torch.zeros_like(x)) for x in (k, v))
+        x = q[at:at + n].double().view(n, H, G, D)
+        sc = torch.einsum("nhgd,hld->hgnl", x, k) * D ** -0.5
+        reach = torch.einsum("nhgd,hld->hgnl", x.abs(), k.abs()).masked_fill(~seen, 0).amax(-1).permute(2, 0, 1)[..., None] * D ** -0.5
+        p = torch.softmax(sc.masked_fill(~seen, -np.inf), -1)
+        want = torch.einsum("hgnl,hld->nhgd", p, v)
+        A = torch.einsum("hgnl,hld->nhgd", p, v.abs())
+        S = torch.einsum("nl,hld->nhd", seen.double(), v.abs())[:, :, None]
+        rel = (2.0 ** -11 if f16 else 2.0 ** -8) + eps / 2 + 2e-4 + 2.0 ** -23 * reach
+        if c.quant_bits:
+            rel = rel + 2.0 ** -11 + 2 * 2.0 ** -11 * reach
+        tol = rel * A + (2.0 ** -32 * S if f16 else 0) + (2.0 ** -25 if dt == orc.F16 else 1e-38)
+        if c.quant_bits and dt == orc.F16:
+            tol = tol + 2.0 ** -25
+        elif c.quant_bits and c.meta_dtype == orc.F32:
+            top = want.abs().unflatten(-1, (-1, min(c.group_size, 32))).amax(-1, keepdim=True)
+            tol = tol + (2.0 ** -25 * (top >= 2.0 ** -13)).expand(*top.shape[:-1], min(c.group_size, 32)).flatten(-2)
+        got = out[at:at + n].double().view(n, H, G, D)
+        assert torch.isfinite(got).all()
+        err = (got - want).abs()
+        assert (err <= tol).all(), (n, L, float((err / tol).max()))
+        at += n
+
+
+@pytest.mark.parametrize("dt,bits,meta", [(orc.F16, 0, orc.F16), (orc.BF16, 0, orc.F16), (orc.BF16, 8, orc.F16), (orc.BF16, 4, orc.F32)])
+@pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 17.5, 20.0])
+@pytest.mark.parametrize("D,q_lens,ctx", [(128, [3, 70], [5000, 900]), (64, [2], [40000])])
+def test_tail_behind_one_key(cuda, dt, bits, meta, gap, D, q_lens, ctx):
+    """The first key holds nearly all the weight and its value is 0: the output is the tail's alone, `gap` nats below.
+    The second shape splits one item over many parts, with the first key in one of them."""
+    H, G, bs = 2, 4, 16
+    lens = [n + c for n, c in zip(q_lens, ctx)]
+    g = torch.Generator("cuda").manual_seed(int(gap * 10) + D)
+    N = sum(-(-n // bs) for n in lens)
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=32, meta_dtype=meta)
+    sign = torch.where(torch.rand(D, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    q = (sign + 0.02 * torch.randn(sum(q_lens), H * G, D, generator=g, device="cuda")).to(TORCH[dt])
+    bt = tables(lens, bs, N, g)
+    slots = torch.arange(N * bs, device="cuda", dtype=torch.int32)
+    k = 0.05 * torch.randn(N * bs, H, D, generator=g, device="cuda")
+    v = 1 + 0.5 * torch.randn(N * bs, H, D, generator=g, device="cuda")
+    for s in range(len(lens)):
+        k[int(bt[s, 0]) * bs] = sign * gap * D ** -0.5
+        v[int(bt[s, 0]) * bs] = 0
+    pool.append(k.to(TORCH[dt]), v.to(TORCH[dt]), slots, N * bs)
+    out = attend(pool, q, G, bt, q_lens, lens)
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, q_lens, lens, out, dt)
