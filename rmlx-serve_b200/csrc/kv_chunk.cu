@@ -616,7 +616,10 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       const int pos = it.t.pos0 + tok;
       const int lim = valid ? max(pos + 1, 0) : INT32_MAX;  // visible keys: low <= key < lim
       const int low = valid && a.window && pos >= a.window ? pos - a.window + 1 : 0;
-      float m = -INFINITY, l = 0.0f, c = a.scale_log2;
+      // A lane without a row scores whatever lies in shared memory: with a maximum
+      // that nothing exceeds it has no say in when the warp moves its rows' maxima,
+      // and the rows' bits do not depend on what ran before.
+      float m = valid ? -INFINITY : INFINITY, l = 0.0f, c = a.scale_log2;
       bool ok = true;
       for (int j = 0; j < mine; ++j) {
         const int b = j & 1;

@@ -98,3 +98,27 @@ def test_tail_behind_one_key(cuda, dt, bits, meta, gap, D, q_lens, ctx):
     out = attend(pool, q, G, bt, q_lens, lens)
     assert pool.check() == 0
     check_rows(pool, q, G, bt, q_lens, lens, out, dt)
+
+
+@pytest.mark.parametrize("dt,bits", [(orc.BF16, 0), (orc.F16, 0), (orc.BF16, 8), (orc.BF16, 4)])
+def test_same_bits_whatever_ran_before(cuda, dt, bits):
+    """The same call after calls that leave other queries in shared memory gives the same bits: 5 tokens of 4 heads
+    fill 20 lanes of a warp's 32, and the others must have no say."""
+    H, G, D, bs = 8, 4, 128, 16
+    g = torch.Generator("cuda").manual_seed(31)
+    q_lens, lens = [5] * 40 + [33], [900 + 37 * i for i in range(41)]
+    N = sum(-(-n // bs) for n in lens)
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=64, meta_dtype=orc.F16)
+    slots = torch.arange(N * bs, device="cuda", dtype=torch.int32)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda").to(TORCH[dt]) for _ in range(2))
+    pool.append(k, v, slots, N * bs)
+    bt = tables(lens, bs, N, g)
+    q = (1.5 * torch.randn(sum(q_lens), H * G, D, generator=g, device="cuda")).to(TORCH[dt])
+    results = []
+    for size in (0.0, 0.5, 4.0, 30.0):
+        before = (size * torch.randn(64 * 41, H * G, D, generator=g, device="cuda")).to(TORCH[dt])
+        attend(pool, before, G, bt, [64] * 41, lens)
+        results.append(attend(pool, q, G, bt, q_lens, lens))
+    assert pool.check() == 0
+    for r in results[1:]:
+        assert torch.equal(results[0].view(torch.int16), r.view(torch.int16))
