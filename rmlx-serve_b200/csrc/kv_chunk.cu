@@ -326,7 +326,7 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 //
 // Quantised pools: codes are dequantised to f16 in shared memory and the
 // products run in f16 (11 bits; bf16's 8 would add more error than the codes),
-// a bf16 query row scaled by a power of two into f16's range.  Groups whose
+// a bf16 query row scaled by a power of two to f16's upper end.  Groups whose
 // values leave f16's range become NaN, and their rows take that path too.
 // Where a box of codes and of (scale, zero) rows is whole 16-byte pieces, one
 // warp fetches them by bulk copies (1-16 tokens over 4-bit pools of 1024-8192
@@ -946,7 +946,8 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
                 for (int o = 1; o < CPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                 e = (int)(__float_as_uint(mx) >> 23);  // 2^(e - 127) <= max
-                if (e == 0 || e == 255) e = 127;       // zeros, infinities
+                // the largest element to 2^14 .. 2^15, so that elements keep their bits down to 2^-28 of it
+                e = e == 0 || e == 255 ? 127 : max(e - 14, 1);  // zeros, infinities: as they are
                 const float inv = 1.0f / __uint_as_float((uint32_t)e << 23);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) q4[i] = pack2<RMLX_F16>(unpack_lo<DT>(q4[i]) * inv, unpack_hi<DT>(q4[i]) * inv);

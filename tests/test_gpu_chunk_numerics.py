@@ -122,3 +122,25 @@ def test_same_bits_whatever_ran_before(cuda, dt, bits):
     assert pool.check() == 0
     for r in results[1:]:
         assert torch.equal(results[0].view(torch.int16), r.view(torch.int16))
+
+
+@pytest.mark.parametrize("bits,meta", [(8, orc.F32), (4, orc.F16)])
+def test_query_rows_of_many_sizes(cuda, bits, meta):
+    """One element of a bf16 query row is 2^23 times the others, and its keys are as much smaller: the small elements
+    decide the scores and keep their eight bits."""
+    H, G, D, bs, dt = 1, 4, 128, 16, orc.BF16
+    g = torch.Generator("cuda").manual_seed(32)
+    L, n = 320, 45
+    pool = rmlx_kv.KVPool(1, H, D, bs, L // bs, dtype=dt, quant_bits=bits, group_size=32, meta_dtype=meta)
+    k, v = (torch.randn(L, H, D, generator=g, device="cuda") for _ in range(2))
+    k[:, :, :32] *= 1e-3
+    k[:, :, 32:] *= 3000
+    pool.append(k.to(TORCH[dt]), v.to(TORCH[dt]), torch.arange(L, device="cuda", dtype=torch.int32), L)
+    q = torch.randn(n, H * G, D, generator=g, device="cuda")
+    q[..., 32:] *= 2.0 ** -9
+    q[..., 5] = 2.0 ** 14
+    q = q.to(TORCH[dt])
+    bt = torch.arange(L // bs, dtype=torch.int32, device="cuda")[None]
+    out = attend(pool, q, G, bt, [n], [310])
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, [n], [310], out, dt)
