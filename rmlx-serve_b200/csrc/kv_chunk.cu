@@ -32,80 +32,6 @@ struct ChunkArgs {
   float scale_log2;
 };
 
-// This lane's head_dim / 32 elements of stored row `row` (K or V) of a tile,
-// dequantised in f32 when the pool holds codes (not rounded to the pool's
-// type: 8 bits of a bf16 value would cost more than the codes' own).
-template <int DT, int HD>
-__device__ __forceinline__ void load_row(const PoolGeo& g, const ChunkArgs& a, const uint8_t* tile, int row, int lane,
-                                         float (&f)[HD / 32]) {
-  constexpr int EPL = HD / 32;
-  const int e0 = lane * EPL;
-  if (a.bits == 0) {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(tile + (int64_t)row * g.row_bytes) + e0;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      if (DT == RMLX_BF16) f[e] = __uint_as_float((uint32_t)__ldg(p + e) << 16);
-      else f[e] = __half2float(__ushort_as_half(__ldg(p + e)));
-    }
-    return;
-  }
-  const uint8_t* codes = tile + (int64_t)row * g.row_bytes;
-  const uint8_t* meta = tile + (int64_t)g.bs * g.row_bytes + (int64_t)row * g.meta_row_bytes;
-  const int q = e0 >> a.gs_log2;
-  float sc, zr;
-  if (a.mf32) {
-    sc = __ldg(reinterpret_cast<const float*>(meta) + 2 * q);
-    zr = __ldg(reinterpret_cast<const float*>(meta) + 2 * q + 1);
-  } else {
-    sc = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const uint16_t*>(meta) + 2 * q)));
-    zr = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const uint16_t*>(meta) + 2 * q + 1)));
-  }
-#pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    const int i = e0 + e;
-    const int c = a.bits == 8 ? __ldg(codes + i) : (__ldg(codes + (i >> 1)) >> (4 * (i & 1))) & 15;
-    f[e] = __fadd_rn(__fmul_rn((float)c, sc), zr);
-  }
-}
-
-// One query row against keys [k0, k1) by one warp, a key at a time, with the
-// running maximum m and sum l of a softmax in the log2 domain; acc is this
-// lane's head_dim / 32 elements of the unnormalised output.  Rows that the
-// mask hides are never read.
-template <int DT, int HD>
-__device__ __forceinline__ void attend_row(const PoolGeo& g, const ChunkArgs& a, const int32_t* btrow, int h, int k0,
-                                           int k1, const float (&qf)[HD / 32], int lane, int32_t* err, float& m,
-                                           float& l, float (&acc)[HD / 32]) {
-  constexpr int EPL = HD / 32;
-  constexpr unsigned FULL = 0xffffffffu;
-  const int64_t vdelta = (int64_t)g.heads * g.tile_bytes;
-  for (int j = k0; j < k1; ++j) {
-    const int b = j / g.bs;
-    const int32_t blk = __ldg(btrow + b);
-    if (blk < 0 || blk >= g.nblocks) {
-      if (lane == 0) atomicOr(err, DEV_ERR_BLOCK);
-      continue;
-    }
-    const uint8_t* tile = g.base + g.tile_off(blk, a.layer, 0, h);
-    float kf[EPL], vf[EPL];
-    load_row<DT, HD>(g, a, tile, j - b * g.bs, lane, kf);
-    load_row<DT, HD>(g, a, tile + vdelta, j - b * g.bs, lane, vf);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) s = fmaf(qf[e], kf[e], s);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
-    s *= a.scale_log2;
-    const float n = fmaxf(m, s);
-    const float base = n == -INFINITY ? 0.0f : n;  // a score of -inf before any other: exp2(-inf - 0) = 0
-    const float f = exp2f(m - base), p = exp2f(s - base);
-    m = n;
-    l = fmaf(l, f, p);
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) acc[e] = fmaf(acc[e], f, p * vf[e]);
-  }
-}
-
 // ---------------------------------------------------------------------------
 // The plan.  A tile is up to 256 query rows of one sequence and KV head: the
 // G query heads of 256 / G consecutive chunk tokens, so that every K/V row
@@ -525,6 +451,207 @@ __device__ __forceinline__ void store_rows64(uint32_t (&w)[16], uint8_t* dst, bo
   }
 }
 
+// This lane's head_dim / 32 elements of U stored rows (K or V) as they lie in
+// memory: plain rows', or codes with the (scale, zero) of their group.
+template <int HD, int BITS, int U>
+struct LaneRows {
+  static constexpr int EPL = HD / 32, BYTES = EPL * (BITS ? BITS : 16) / 8;
+  uint32_t w[U][BYTES == 8 ? 2 : 1];
+  uint2 meta[U];
+  // tile[u]: the tile of row u (slot row[u] of its block)
+  __device__ __forceinline__ void load(const PoolGeo& g, const ChunkArgs& a, const uint8_t* const (&tile)[U],
+                                       const int (&row)[U], int lane) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint8_t* p = tile[u] + (int64_t)row[u] * g.row_bytes + lane * BYTES;
+      if constexpr (BYTES == 8) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+        w[u][0] = x.x, w[u][1] = x.y;
+      } else if constexpr (BYTES == 4) {
+        w[u][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      } else if constexpr (BYTES == 2) {
+        w[u][0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+      } else {
+        w[u][0] = __ldg(p);
+      }
+    }
+    if constexpr (BITS != 0) {
+      const int q = (lane * EPL) >> a.gs_log2;
+      auto at = [&](int u) { return tile[u] + (int64_t)g.bs * g.row_bytes + (int64_t)row[u] * g.meta_row_bytes; };
+      if (a.mf32) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) meta[u] = __ldg(reinterpret_cast<const uint2*>(at(u)) + q);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t m = __ldg(reinterpret_cast<const uint32_t*>(at(u)) + q);
+          meta[u] = make_uint2(__float_as_uint(unpack_lo<RMLX_F16>(m)), __float_as_uint(unpack_hi<RMLX_F16>(m)));
+        }
+      }
+    }
+  }
+  // Row u in f32; codes are not rounded to the pool's type (8 bits of a bf16 value would cost more than the codes' own).
+  template <int DT>
+  __device__ __forceinline__ void get(int u, float (&f)[EPL]) const {
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      if constexpr (BITS == 0)
+        f[e] = (e & 1) ? unpack_hi<DT>(w[u][e >> 1]) : unpack_lo<DT>(w[u][e >> 1]);
+      else
+        f[e] = __fadd_rn(__fmul_rn((float)((w[u][0] >> (BITS * e)) & ((1u << BITS) - 1)), __uint_as_float(meta[u].x)),
+                         __uint_as_float(meta[u].y));
+    }
+  }
+};
+
+// What a warp's lanes know of an item's portion whose rows are computed again.
+struct AgainRows {
+  const int32_t* btrow;
+  float* part;            // where a portion's partial rows go, nullptr when the rows are whole
+  int64_t token0, orow;   // first chunk token of the tile in q; this lane's row in out
+  int head, k_first, k_end;
+  int row, lim, low;      // this lane's row of the tile: it sees keys low <= key < lim
+};
+
+// The exact path: the rows of the lanes in `bad` again in f32, four rows and four
+// keys at a time by the whole warp, with the running maximum and sum of a softmax
+// in the log2 domain.  A row that none of the four sees is never read, and one that
+// a row's mask hides has no part in that row.  Lane 4 r + u ends up with the score
+// of row r and key u (15 shuffles for 16 sums over the lanes, and one that joins the
+// warp's halves) and keeps its row's maximum and its own share of the sum.  Bound
+// by instruction issue: about 100 ns a row and key in each of eight warps (82 of a
+// plain pool); a row and a key at a time took 950.  Out of line, and four keys
+// instead of eight, so that its registers are not the main loop's.
+template <int DT, int HD, int BITS>
+__device__ __noinline__ void attend_rows_again(const ChunkParams& p, const AgainRows& it, unsigned bad, int32_t* err) {
+  constexpr int EPL = HD / 32, R = 4, U = 4;
+  constexpr unsigned FULL = 0xffffffffu;
+  const PoolGeo& g = p.g;
+  const ChunkArgs& a = p.a;
+  const int lane = threadIdx.x & 31, u_own = lane % U, r_own = lane / U % R;
+  const int64_t vdelta = (int64_t)g.heads * g.tile_bytes;
+  auto block_of = [&](int j) { return a.bs_log2 >= 0 ? j >> a.bs_log2 : j / g.bs; };
+  bool out_of_pool = false;
+#pragma unroll 1
+  while (bad) {
+    int from[R], n = 0;  // the lanes whose rows are taken; a last row stands in for missing ones
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (bad) {
+        from[r] = __ffs(bad) - 1, bad &= bad - 1, ++n;
+      } else {
+        from[r] = from[r ? r - 1 : 0];
+      }
+    }
+    float q[R][EPL], acc[R][EPL];
+    int k0 = INT32_MAX, k1 = 0, own0 = 0, own1 = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = __shfl_sync(FULL, it.row, from[r]);
+      const int r0 = max(__shfl_sync(FULL, it.low, from[r]), it.k_first), r1 = min(__shfl_sync(FULL, it.lim, from[r]), it.k_end);
+      k0 = min(k0, r0), k1 = max(k1, r1);
+      if (r == r_own) own0 = r0, own1 = r1;
+      const int tok = row / a.G;
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q + (it.token0 + tok) * a.qts +
+                                                             (it.head * a.G + row - tok * a.G) * a.qhs) + lane * EPL;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) q[r][e] = unpack_lo<DT>(__ldg(qp + e)), acc[r][e] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+    for (int j0 = k0; j0 < k1; j0 += U) {
+      const uint8_t* tile[U];
+      int slot[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = min(j0 + u, k1 - 1), b = block_of(j);
+        const int32_t blk = __ldg(it.btrow + b);
+        const bool good = blk >= 0 && blk < g.nblocks;
+        out_of_pool |= !good;
+        tile[u] = g.base + g.tile_off(good ? blk : 0, a.layer, 0, it.head);
+        slot[u] = j - b * g.bs;
+      }
+      LaneRows<HD, BITS, U> kr, vr;
+      kr.load(g, a, tile, slot, lane);
+      float s[R * U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[EPL];
+        kr.template get<DT>(u, f);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          s[r * U + u] = 0.0f;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) s[r * U + u] = fmaf(q[r][e], f[e], s[r * U + u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) tile[u] += vdelta;
+      vr.load(g, a, tile, slot, lane);
+#pragma unroll
+      for (int o = R * U / 2; o; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+          const float keep = up ? s[i + o] : s[i], give = up ? s[i] : s[i + o];
+          s[i] = keep + __shfl_xor_sync(FULL, give, o);
+        }
+      }
+#pragma unroll
+      for (int o = R * U; o < 32; o <<= 1) s[0] += __shfl_xor_sync(FULL, s[0], o);
+      const bool sees = j0 + u_own >= own0 && j0 + u_own < own1;
+      const float x = sees ? s[0] * a.scale_log2 : -INFINITY;
+      float top = x;
+#pragma unroll
+      for (int o = U / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+      top = fmaxf(top, m);
+      const float base = top == -INFINITY ? 0.0f : top;  // scores of -inf before any other: exp2(-inf - 0) = 0
+      const float f = exp2f(m - base), w = exp2f(x - base);
+      m = top;
+      l = fmaf(l, f, w);
+      const float mine = sees ? w : -1.0f;  // below 0: hidden, whatever the row holds
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float fr = __shfl_sync(FULL, f, r * U);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[r][e] *= fr;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[EPL];
+        vr.template get<DT>(u, v);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float pr = __shfl_sync(FULL, mine, r * U + u);
+          const bool use = !(pr < 0.0f);  // NaN counts
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[r][e] = use ? fmaf(pr, v[e], acc[r][e]) : acc[r][e];
+        }
+      }
+    }
+#pragma unroll
+    for (int o = U / 2; o; o >>= 1) l += __shfl_xor_sync(FULL, l, o);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float rl = __shfl_sync(FULL, l, r * U), rm = __shfl_sync(FULL, m, r * U);
+      const int row = __shfl_sync(FULL, it.row, from[r]);
+      const int64_t orow = __shfl_sync(FULL, it.orow, from[r]);
+      if (r >= n) continue;
+      if (it.part) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) it.part[(size_t)(lane * EPL + e) * CH_ROWS + row] = acc[r][e];
+        if (lane == 0) reinterpret_cast<float2*>(it.part + (size_t)CH_ROWS * HD)[row] = make_float2(rm, rl);
+      } else {
+        const float il = rl == 0.0f ? 0.0f : 1.0f / rl;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+          reinterpret_cast<uint16_t*>(a.out)[orow * HD + lane * EPL + e] = (uint16_t)pack2<DT>(acc[r][e] * il, 0.0f);
+      }
+    }
+  }
+  if (out_of_pool && lane == 0) atomicOr(err, DEV_ERR_BLOCK);
+}
+
 template <int DT, int HD, int BITS, bool TMA>
 __global__ void __launch_bounds__(ch_threads(TMA), 1)
     chunk_attn_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map, int32_t* err) {
@@ -758,33 +885,15 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         }
         if (valid && !whole) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[row] = make_float2(ml, l);
         // rows whose output holds NaN: again, from visible rows only
-        unsigned bad = __ballot_sync(0xffffffffu, valid && nan != nan);
-        while (bad) {
-          const int b = __ffs(bad) - 1;
-          bad &= bad - 1;
-          const int br = __shfl_sync(0xffffffffu, row, b), blim = __shfl_sync(0xffffffffu, lim, b),
-                    blow = __shfl_sync(0xffffffffu, low, b);
-          const int64_t bo = __shfl_sync(0xffffffffu, orow, b);
-          const int bt = br / a.G, bg = br - bt * a.G;
-          constexpr int EPL = HD / 32;
-          float qf[EPL], acc[EPL], bm = -INFINITY, bl = 0.0f;
-          const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q + (it.qoff + it.t.t0 + bt) * a.qts +
-                                                                 (it.head * a.G + bg) * a.qhs) + lane * EPL;
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) qf[e] = unpack_lo<DT>(__ldg(qp + e)), acc[e] = 0.0f;
-          const int k_first = (it.t.k_lo + it.k0) * CH_KEYS, k_end = (it.t.k_lo + it.k1) * CH_KEYS;
-          attend_row<DT, HD>(g, a, a.bt + (int64_t)it.s * a.bt_stride, it.head, max(blow, k_first), min(blim, k_end),
-                             qf, lane, err, bm, bl, acc);
-          const float bi = whole ? (bl == 0.0f ? 0.0f : 1.0f / bl) : 1.0f;
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) {
-            const float y = acc[e] * bi;
-            if (whole)
-              reinterpret_cast<uint16_t*>(p.a.out)[bo * HD + lane * EPL + e] = (uint16_t)pack2<DT>(y, 0.0f);
-            else
-              part[(size_t)(lane * EPL + e) * CH_ROWS + br] = y;
-          }
-          if (!whole && lane == 0) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[br] = make_float2(bm, bl);
+        const unsigned bad = __ballot_sync(0xffffffffu, valid && nan != nan);
+        if (bad) {
+          AgainRows again;
+          again.btrow = a.bt + (int64_t)it.s * a.bt_stride;
+          again.part = whole ? nullptr : part;
+          again.token0 = it.qoff + it.t.t0, again.orow = orow, again.head = it.head;
+          again.k_first = (it.t.k_lo + it.k0) * CH_KEYS, again.k_end = (it.t.k_lo + it.k1) * CH_KEYS;
+          again.row = row, again.lim = lim, again.low = low;
+          attend_rows_again<DT, HD, BITS>(p, again, bad, err);
         }
         tc_fence_before();
       }

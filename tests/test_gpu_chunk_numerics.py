@@ -144,3 +144,59 @@ def test_query_rows_of_many_sizes(cuda, bits, meta):
     out = attend(pool, q, G, bt, [n], [310])
     assert pool.check() == 0
     check_rows(pool, q, G, bt, [n], [310], out, dt)
+
+
+def event_ms(f, n=3):
+    f()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    a.record()
+    for _ in range(n):
+        f()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b) / n
+
+
+@pytest.mark.parametrize("dt,bits", [(orc.BF16, 0), (orc.F16, 0), (orc.BF16, 8)])
+@pytest.mark.parametrize("D,n,L", [(128, 60, 100), (128, 60, 2000), (64, 3, 20000)])
+def test_rows_computed_again_repeat(cuda, dt, bits, D, n, L):
+    """NaN in the last row, which the mask hides from all tokens but the last: their rows are computed again, in whole
+    items (100 rows) and in parts, and come back finite, right and the same every time."""
+    H, G, bs = 2, 4, 16
+    g = torch.Generator("cuda").manual_seed(37)
+    N = -(-L // bs)
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=32, meta_dtype=orc.F32)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda") for _ in range(2))
+    v[L - 1] = float("nan")
+    pool.append(k.to(TORCH[dt]), v.to(TORCH[dt]), torch.arange(N * bs, device="cuda", dtype=torch.int32), N * bs)
+    bt = torch.arange(N, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(n, H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    first = attend(pool, q, G, bt, [n], [L])
+    for _ in range(10):
+        assert torch.equal(attend(pool, q, G, bt, [n], [L]).view(torch.int16), first.view(torch.int16))
+    assert pool.check() == 0
+    assert torch.isnan(first[-1]).all()
+    check_rows(pool, q[:-1], G, bt, [n - 1], [L - 1], first[:-1], dt)
+
+
+@pytest.mark.parametrize("bits", [0, 8])
+def test_rows_computed_again_in_time(cuda, bits):
+    """Every row of the last tile over 8192 keys through the exact path: some 75 to 100 times as long as a call
+    without (a row and a key at a time took 700 times as long, and a million keys ran into the waits' limit)."""
+    H, G, D, bs, dt, n, L = 8, 4, 128, 16, orc.BF16, 512, 8192
+    g = torch.Generator("cuda").manual_seed(38)
+    k, v = (torch.randn(L, H, D, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(n, H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    bt = torch.arange(L // bs, dtype=torch.int32, device="cuda")[None]
+    ms = []
+    for junk in (False, True):
+        if junk:
+            v[L - 1] = float("nan")
+        pool = rmlx_kv.KVPool(1, H, D, bs, L // bs, dtype=dt, quant_bits=bits, group_size=64, meta_dtype=orc.F32)
+        pool.append(k.to(TORCH[dt]), v.to(TORCH[dt]), torch.arange(L, device="cuda", dtype=torch.int32), L)
+        ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(q)
+        ms.append(event_ms(lambda: attend(pool, q, G, bt, [n], [L], out, ws)))
+        assert pool.check() == 0
+    assert torch.isfinite(out[:-1]).all() and torch.isnan(out[-1]).all()
+    assert ms[1] <= 250 * ms[0], ms
