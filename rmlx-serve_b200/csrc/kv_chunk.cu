@@ -887,6 +887,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         // rows whose output holds NaN: again, from visible rows only
         const unsigned bad = __ballot_sync(0xffffffffu, valid && nan != nan);
         if (bad) {
+          __syncwarp();  // other lanes store these rows again: behind what this lane has stored of them
           AgainRows again;
           again.btrow = a.bt + (int64_t)it.s * a.bt_stride;
           again.part = whole ? nullptr : part;

@@ -179,6 +179,22 @@ def test_rows_computed_again_repeat(cuda, dt, bits, D, n, L):
     check_rows(pool, q[:-1], G, bt, [n - 1], [L - 1], first[:-1], dt)
 
 
+def test_no_first_store_outlives_the_second(cuda):
+    """Every row of many whole items is stored twice, first as NaN by one lane and then by others: no NaN is left."""
+    H, G, D, bs, dt, S = 8, 16, 128, 16, orc.BF16, 64
+    g = torch.Generator("cuda").manual_seed(39)
+    pool = rmlx_kv.KVPool(1, H, D, bs, S * 2, dtype=dt)
+    k, v = (torch.randn(S * 32, H, D, generator=g, device="cuda") for _ in range(2))
+    v[31::32] = float("nan")
+    pool.append(k.to(TORCH[dt]), v.to(TORCH[dt]), torch.arange(S * 32, device="cuda", dtype=torch.int32), S * 32)
+    bt = torch.arange(S * 2, dtype=torch.int32, device="cuda").view(S, 2)
+    q = torch.randn(S * 16, H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    for _ in range(5):
+        out = attend(pool, q, G, bt, [16] * S, [32] * S).view(S, 16, H * G, D)
+        assert torch.isfinite(out[:, :15]).all() and torch.isnan(out[:, 15]).all()
+    assert pool.check() == 0
+
+
 @pytest.mark.parametrize("bits", [0, 8])
 def test_rows_computed_again_in_time(cuda, bits):
     """Every row of the last tile over 8192 keys through the exact path: some 75 to 100 times as long as a call
