@@ -278,9 +278,9 @@ struct ChunkSmem {
   static constexpr int UNITS = BITS ? CH_KEYS * HD * BITS / 128 : 0;  // of a tile
   static constexpr int RAW_BYTES = BITS == 8 ? UNITS * 60 : UNITS * 96;
   static constexpr int Q = 0, KV = 2 * QTILE, RAW = KV + STAGES * STAGE, CTRL = RAW + RAW_BYTES;
-  // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales
-  static constexpr int BARS = CTRL, PLAN = CTRL + 352, ML = PLAN + 128, QSCALE = ML + 1024;
-  static constexpr int BYTES = QSCALE + 512;
+  // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales, items with tiny groups
+  static constexpr int BARS = CTRL, PLAN = CTRL + 352, ML = PLAN + 128, QSCALE = ML + 1024, TINY = QSCALE + 512;
+  static constexpr int BYTES = TINY + 64;
 };
 // barrier numbers
 constexpr int BAR_FULL = 0, BAR_EMPTY = 8, BAR_QFULL = 16, BAR_QEMPTY = 17, BAR_OFREE = 18, BAR_ML = 19, BAR_O = 20,
@@ -375,22 +375,24 @@ __device__ __forceinline__ uint2 load_meta(const uint8_t* meta, int q, bool mf32
   return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(meta) + q), 0u);
 }
 // A group's scale and zero as the conversion takes them.  Its values lie
-// between zr and zr + qmax sc: where they leave f16's range, or where the
-// largest is below 2^-13, so that f16's smallest step (rounding 2^-25) would
-// cost more than 2^-12 of it, the scale becomes NaN, and the rows that see the
-// group take the exact path.
+// between zr and zr + qmax sc: where they leave f16's range the scale becomes NaN,
+// and the rows that see the group take the exact path.  True when the group is
+// tiny: its largest value is below 2^-13, where f16's smallest step (a rounding of
+// 2^-25) costs more than 2^-12 of it.  With f16 scales and zeros none is: all
+// values are multiples of 2^-24, and those below 2^-13 are f16 numbers.
 template <int BITS>
 struct Group {
   float sc, zr;
   __half2 sc2, zr2;
-  __device__ __forceinline__ void set(uint2 meta, bool mf32) {
+  __device__ __forceinline__ bool set(uint2 meta, bool mf32) {
     float s = mf32 ? __uint_as_float(meta.x) : unpack_lo<RMLX_F16>(meta.x);
     const float z = mf32 ? __uint_as_float(meta.y) : unpack_hi<RMLX_F16>(meta.x);
     const float top = fmaxf(fabsf(z), fabsf(fmaf((float)((1 << BITS) - 1), s, z)));
     const float least = s == 1.0f ? fabsf(z) : top;  // a flat group has scale 1 and no code but 0
-    if (!(top <= 65504.0f) || (least > 0.0f && least < 1.220703125e-4f)) s = __uint_as_float(0x7fffffffu);
+    if (!(top <= 65504.0f)) s = __uint_as_float(0x7fffffffu);
     sc = s, zr = z;
     sc2 = __float2half2_rn(s), zr2 = __float2half2_rn(z);
+    return mf32 && least > 0.0f && least < 1.220703125e-4f;
   }
 };
 // Eight elements as f16 pairs from their codes, a byte each.  A code becomes
@@ -677,7 +679,10 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
   ItemIter* plan = reinterpret_cast<ItemIter*>(smem + S::PLAN);
   float2* ml_b = reinterpret_cast<float2*>(smem + S::ML);
   uint8_t* qscale = smem + S::QSCALE;  // [2][CH_ROWS] f32 exponents, by item parity
+  // [K, V][item % 8]: number, from 1, of an item with a tiny group there (loads run at most four items ahead of an epilogue)
+  volatile uint32_t* tiny = reinterpret_cast<volatile uint32_t*>(smem + S::TINY);
 
+  if (threadIdx.x < 16) tiny[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < ST; ++i) {
@@ -850,6 +855,14 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         tc_fence_after();
         const float il = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
         float nan = l;  // becomes NaN with any NaN among the outputs
+        // Tiny groups lie in f16 with an error of up to 2^-25.  In V that is more than
+        // 2^-12 of a group's largest output where this is below 2^-13: such a row is
+        // computed again (f16 outputs are rounded by 2^-25 themselves).  In K it moves a
+        // score by 2^-25 scale sum |q|, at most 2^-12 unless head_dim times the row's
+        // largest element (below 2^15 in units of c) is above 2^13 / scale.
+        const bool tiny_v = BITS && DT == RMLX_BF16 && tiny[8 + ((nitem - 1) & 7)] == nitem;
+        const float faint = (whole ? 1.0f : l) * 1.220703125e-4f;
+        bool again = BITS && tiny[(nitem - 1) & 7] == nitem && c * HD > 0.25f * 1.4426950408889634f;
 #pragma unroll 1
         for (int i = 0; i < HD; i += 32) {
           uint32_t o[32];
@@ -873,6 +886,18 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             f[e] = l == 0.0f ? 0.0f : f[e] * il;
             nan = fmaf(f[e], 0.0f, nan);
           }
+          if (tiny_v) {  // the largest of each group's columns, or of these 32
+            float top[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              top[k] = fabsf(f[8 * k]);
+#pragma unroll
+              for (int e = 1; e < 8; ++e) top[k] = fmaxf(top[k], fabsf(f[8 * k + e]));
+            }
+            if (a.gs_log2 > 3) top[0] = top[1] = fmaxf(top[0], top[1]), top[2] = top[3] = fmaxf(top[2], top[3]);
+            if (a.gs_log2 > 4) top[0] = top[1] = top[2] = top[3] = fmaxf(top[0], top[2]);
+            again |= fminf(fminf(top[0], top[1]), fminf(top[2], top[3])) < faint;
+          }
           if (whole) {
             uint32_t w[16];
 #pragma unroll
@@ -884,17 +909,17 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           }
         }
         if (valid && !whole) reinterpret_cast<float2*>(part + (size_t)CH_ROWS * HD)[row] = make_float2(ml, l);
-        // rows whose output holds NaN: again, from visible rows only
-        const unsigned bad = __ballot_sync(0xffffffffu, valid && nan != nan);
+        // rows whose output holds NaN, or too few digits: again, from visible rows only
+        const unsigned bad = __ballot_sync(0xffffffffu, valid && (nan != nan || again));
         if (bad) {
           __syncwarp();  // other lanes store these rows again: behind what this lane has stored of them
-          AgainRows again;
-          again.btrow = a.bt + (int64_t)it.s * a.bt_stride;
-          again.part = whole ? nullptr : part;
-          again.token0 = it.qoff + it.t.t0, again.orow = orow, again.head = it.head;
-          again.k_first = (it.t.k_lo + it.k0) * CH_KEYS, again.k_end = (it.t.k_lo + it.k1) * CH_KEYS;
-          again.row = row, again.lim = lim, again.low = low;
-          attend_rows_again<DT, HD, BITS>(p, again, bad, err);
+          AgainRows rows;
+          rows.btrow = a.bt + (int64_t)it.s * a.bt_stride;
+          rows.part = whole ? nullptr : part;
+          rows.token0 = it.qoff + it.t.t0, rows.orow = orow, rows.head = it.head;
+          rows.k_first = (it.t.k_lo + it.k0) * CH_KEYS, rows.k_end = (it.t.k_lo + it.k1) * CH_KEYS;
+          rows.row = row, rows.lim = lim, rows.low = low;
+          attend_rows_again<DT, HD, BITS>(p, rows, bad, err);
         }
         tc_fence_before();
       }
@@ -1046,22 +1071,19 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               const int r = r0 + u * step;
-              int e = 127;  // the row's power of two, and a bf16 row in f16
-              if (DT == RMLX_BF16) {
-                uint32_t* q4 = reinterpret_cast<uint32_t*>(&w[u]);
-                float mx = 0.0f;
+              // the row in f16, its largest element scaled by a power of two to 2^14 .. 2^15
+              // (the others keep their bits down to 2^-28 of it)
+              uint32_t* q4 = reinterpret_cast<uint32_t*>(&w[u]);
+              float mx = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  mx = fmaxf(mx, fmaxf(fabsf(unpack_lo<DT>(q4[i])), fabsf(unpack_hi<DT>(q4[i]))));
+              for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(unpack_lo<DT>(q4[i])), fabsf(unpack_hi<DT>(q4[i]))));
 #pragma unroll
-                for (int o = 1; o < CPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                e = (int)(__float_as_uint(mx) >> 23);  // 2^(e - 127) <= max
-                // the largest element to 2^14 .. 2^15, so that elements keep their bits down to 2^-28 of it
-                e = e == 0 || e == 255 ? 127 : max(e - 14, 1);  // zeros, infinities: as they are
-                const float inv = 1.0f / __uint_as_float((uint32_t)e << 23);
+              for (int o = 1; o < CPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              int e = (int)(__float_as_uint(mx) >> 23);  // 2^(e - 127) <= max
+              e = e == 255 ? 127 : max(e - 14, 1);       // infinities: as they are
+              const float inv = 1.0f / __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q4[i] = pack2<RMLX_F16>(unpack_lo<DT>(q4[i]) * inv, unpack_hi<DT>(q4[i]) * inv);
-              }
+              for (int i = 0; i < 4; ++i) q4[i] = pack2<RMLX_F16>(unpack_lo<DT>(q4[i]) * inv, unpack_hi<DT>(q4[i]) * inv);
               if (ch == 0 && r < CH_ROWS) qscale[(nitem & 1) * CH_ROWS + r] = (uint8_t)e;
               if (r < it.t.rows) sts128(sb + S::Q + (r >> 7) * S::QTILE + q_off<HD>(r & 127, ch), w[u]);
             }
@@ -1163,6 +1185,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
               };
               uint4 ws[N];
               uint2 sz[N];
+              bool small = false;
 #pragma unroll
               for (int y = 0; y < N; ++y)
                 if (there(y)) ws[y] = lds128(dst + unit(y) * 16), sz[y] = pair(y, 0);
@@ -1173,17 +1196,18 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
                 const bool live = kb + row < it.t.hi;  // else zeros: behind the last visible row
                 const uint32_t cw[4] = {ws[y].x, ws[y].y, ws[y].z, ws[y].w};
                 Group<BITS ? BITS : 8> grp;
-                grp.set(live ? sz[y] : make_uint2(0u, 0u), MF32);
+                small |= grp.set(live ? sz[y] : make_uint2(0u, 0u), MF32);
                 uint4 o[EPU / 8];
 #pragma unroll
                 for (int e = 0; e < EPU / 8; ++e) {
-                  if (!decltype(one)::value && e > 0) grp.set(live ? pair(y, 8 * e) : make_uint2(0u, 0u), MF32);
+                  if (!decltype(one)::value && e > 0) small |= grp.set(live ? pair(y, 8 * e) : make_uint2(0u, 0u), MF32);
                   o[e] = dequant8<BITS ? BITS : 8, MF32>(
                       BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
                 }
 #pragma unroll
                 for (int e = 0; e < EPU / 8; ++e) sts128(out + kv_off<HD>(row, ch * (EPU / 8) + e), o[e]);
               }
+              if (MF32 && small) tiny[8 * kv + ((nitem - 1) & 7)] = nitem;
             };
             const bool one = (1 << a.gs_log2) >= EPU;
             if (!a.mf32 && one) convert(std::false_type(), std::true_type());
@@ -1258,6 +1282,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           constexpr bool MF32 = decltype(mf32)::value;
           int j, kv;
           which(i, j, kv);
+          bool small = false;
 #pragma unroll
           for (int y = 0; y < N; ++y) {
             const int u = u0 + y * 7 * 32;
@@ -1265,8 +1290,8 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             const uint4 w = lds128(sb + S::RAW + (slot * UNITS + u) * 16);
             const uint32_t cw[4] = {w.x, w.y, w.z, w.w};
             Group<BITS ? BITS : 8> grp;
-            grp.set(MF32 ? lds64(raw_meta + (slot * UNITS + u) * 8) : make_uint2(lds32(raw_meta + (slot * UNITS + u) * 4), 0u),
-                    MF32);
+            small |= grp.set(MF32 ? lds64(raw_meta + (slot * UNITS + u) * 8) : make_uint2(lds32(raw_meta + (slot * UNITS + u) * 4), 0u),
+                             MF32);
             const uint8_t* meta = nullptr;
             if (!decltype(one)::value) {
               const int t = key_of(j, y);
@@ -1280,7 +1305,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
             for (int e = 0; e < EPU / 8; ++e) {
               if (!decltype(one)::value && e > 0 && meta)
-                grp.set(load_meta(meta, (ch * EPU + 8 * e) >> a.gs_log2, MF32), MF32);
+                small |= grp.set(load_meta(meta, (ch * EPU + 8 * e) >> a.gs_log2, MF32), MF32);
               o[e] = dequant8<BITS ? BITS : 8, MF32>(
                   BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
             }
@@ -1288,6 +1313,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             for (int e = 0; e < EPU / 8; ++e)
               sts128(sb + S::KV + stage * S::STAGE + kv_off<HD>(u / UPR, ch * (EPU / 8) + e), o[e]);
           }
+          if (MF32 && small) tiny[8 * kv + ((nitem - 1) & 7)] = nitem;
         };
         auto convert = [&](int i, uint32_t stage, int slot) {
           const bool one = (1 << a.gs_log2) >= EPU;

@@ -157,6 +157,74 @@ def event_ms(f, n=3):
     return a.elapsed_time(b) / n
 
 
+@pytest.mark.parametrize("dt,bits,meta", [(orc.BF16, 8, orc.F32), (orc.BF16, 4, orc.F16), (orc.F16, 8, orc.F32)])
+@pytest.mark.parametrize("what", ["v", "k"])
+def test_one_tiny_group_costs_little(cuda, dt, bits, meta, what):
+    """One group of values below f16's normal numbers, in one row that every token sees: right, and at the speed of
+    a call without it (a tenth of it at least; every row taking the exact path is some hundred times slower)."""
+    H, G, D, bs = 4, 4, 128, 16
+    g = torch.Generator("cuda").manual_seed(33)
+    q_lens, lens = [300, 40], [4000, 2000]
+    N = sum(-(-n // bs) for n in lens)
+    bt = tables(lens, bs, N, g)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(sum(q_lens), H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    ms = []
+    for tiny in (False, True):
+        pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=32, meta_dtype=meta)
+        kk, vv = k.clone(), v.clone()
+        if tiny:
+            for s in range(2):
+                (vv if what == "v" else kk)[int(bt[s, 3]) * bs + 5, :, 32:64] *= 2e-5
+        pool.append(kk.to(TORCH[dt]), vv.to(TORCH[dt]), torch.arange(N * bs, device="cuda", dtype=torch.int32), N * bs)
+        ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(q)
+        ms.append(event_ms(lambda: attend(pool, q, G, bt, q_lens, lens, out, ws)))
+        assert pool.check() == 0
+        check_rows(pool, q, G, bt, q_lens, lens, out, dt)
+    assert ms[1] <= 10 * ms[0] + 0.2, ms
+
+
+@pytest.mark.parametrize("dt,bits,meta,gs", [(orc.BF16, 8, orc.F32, 8), (orc.BF16, 4, orc.F32, 16), (orc.BF16, 8, orc.F32, 64),
+                                             (orc.F16, 4, orc.F32, 32), (orc.BF16, 8, orc.F16, 32)])
+@pytest.mark.parametrize("size", [1e-4, 3e-6, 1e-9])
+@pytest.mark.parametrize("D,q_lens,lens", [(128, [40, 3], [310, 90]), (64, [2], [9000])])
+def test_tiny_columns(cuda, dt, bits, meta, gs, size, D, q_lens, lens):
+    """V columns of one group hold tiny values in every key, next to ordinary ones: each output keeps its own digits."""
+    if meta == orc.F16 or dt == orc.F16:
+        size = max(size, 3e-6)  # 1e-9 is 0 in f16
+    H, G, bs = 2, 4, 16
+    g = torch.Generator("cuda").manual_seed(34)
+    N = sum(-(-n // bs) for n in lens)
+    bt = tables(lens, bs, N, g)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda") for _ in range(2))
+    v[:, :, gs * 1 % D:gs * 1 % D + gs] *= size
+    if gs < D:
+        v[:, 1, :gs] = 0  # all zero: no digits to keep
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=gs, meta_dtype=meta)
+    pool.append(k.to(TORCH[dt]), v.to(TORCH[dt]), torch.arange(N * bs, device="cuda", dtype=torch.int32), N * bs)
+    q = torch.randn(sum(q_lens), H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    out = attend(pool, q, G, bt, q_lens, lens)
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, q_lens, lens, out, dt)
+
+
+@pytest.mark.parametrize("dt,kscale,qscale", [(orc.BF16, 1e-5, 1e5), (orc.BF16, 1e-8, 1e8), (orc.F16, 2e-5, 3e4), (orc.BF16, 1e-5, 1e3)])
+def test_tiny_keys_under_large_queries(cuda, dt, kscale, qscale):
+    """Scores of order 1 (and of 0.01) from keys that f16 holds badly or not at all."""
+    H, G, D, bs = 2, 4, 128, 16
+    g = torch.Generator("cuda").manual_seed(35)
+    L, n = 320, 45
+    pool = rmlx_kv.KVPool(1, H, D, bs, L // bs, dtype=dt, quant_bits=8, group_size=32, meta_dtype=orc.F32)
+    k, v = (torch.randn(L, H, D, generator=g, device="cuda") for _ in range(2))
+    pool.append((k * kscale).to(TORCH[dt]), v.to(TORCH[dt]), torch.arange(L, device="cuda", dtype=torch.int32), L)
+    q = (torch.randn(n, H * G, D, generator=g, device="cuda").clamp(-2, 2) * qscale).to(TORCH[dt])
+    bt = torch.arange(L // bs, dtype=torch.int32, device="cuda")[None]
+    out = attend(pool, q, G, bt, [n], [310])
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, [n], [310], out, dt)
+
+
 @pytest.mark.parametrize("dt,bits", [(orc.BF16, 0), (orc.F16, 0), (orc.BF16, 8)])
 @pytest.mark.parametrize("D,n,L", [(128, 60, 100), (128, 60, 2000), (64, 3, 20000)])
 def test_rows_computed_again_repeat(cuda, dt, bits, D, n, L):
