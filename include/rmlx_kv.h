@@ -422,8 +422,9 @@ RMLX_API rmlx_status rmlx_kv_decode_attention(rmlx_kv_pool* p, int32_t layer, co
  * seq_lens[s] rows, the last q_lens[s] of them its chunk; chunk token i
  * stands at position p = seq_lens[s] - q_lens[s] + i and sees rows j <= p,
  * with window > 0 only j > p - window.  A token that sees no row (p < 0) gives
- * zeros; masked rows have no influence whatever they hold.  Sequences of
- * length 0 in q_lens take no rows of q.
+ * zeros; masked rows have no influence whatever they hold, and a block none
+ * of whose rows is seen is not read: its table entry may be anything.
+ * Sequences of length 0 in q_lens take no rows of q.
  * q: rows of all chunks back to back, num_q_tokens of them at least; row
  * (token, query head) at element token * q_token_stride + head *
  * q_head_stride.  out: [token][num_kv_heads * q_heads_per_kv][head_dim] in the

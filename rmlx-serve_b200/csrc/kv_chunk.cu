@@ -62,7 +62,7 @@ constexpr float CH_BIAS = CT == RMLX_F16 ? 7.0f : 0.0f;
 
 // Chunk token range, key tiles and masks of tile mt of a sequence.
 struct TileGeo {
-  int t0, rows, pos0, k_lo, nk, hi;  // first token, rows, its position, first key tile, key tiles, keys end (exclusive)
+  int t0, rows, pos0, k_lo, nk, lo, hi;  // first token, rows, its position, first key tile, key tiles, keys [lo, hi)
 };
 __device__ __forceinline__ TileGeo tile_geo(int qlen, int len, int mt, int tpt, int G, int window) {
   TileGeo t;
@@ -71,8 +71,8 @@ __device__ __forceinline__ TileGeo tile_geo(int qlen, int len, int mt, int tpt, 
   t.rows = n * G;
   t.pos0 = len - qlen + t.t0;
   t.hi = t.pos0 + n;
-  const int lo = window && t.pos0 >= window ? t.pos0 - window + 1 : 0;
-  t.k_lo = lo / CH_KEYS;
+  t.lo = window && t.pos0 >= window ? t.pos0 - window + 1 : 0;
+  t.k_lo = t.lo / CH_KEYS;
   t.nk = t.hi > 0 ? (t.hi - 1) / CH_KEYS + 1 - t.k_lo : 0;
   return t;
 }
@@ -262,7 +262,7 @@ struct ChunkParams {
   PoolGeo g;
   ChunkArgs a;
   int tpt;                 // chunk tokens of a tile
-  int box;                 // rows of a TMA box, or of a bulk copy of codes
+  int box;                 // rows of a TMA box, or of a bulk copy of codes: a power of two
   int raw_depth;           // tiles of codes in flight by bulk copies, 0: codes are copied by the load warps
   float* parts;
   PartDesc* desc;
@@ -1111,8 +1111,10 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
           ++n;
           // one box of p.box rows a lane
-          const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS, t = kb + lane * p.box;
-          const bool want = lane * p.box < CH_KEYS && t < it.t.hi;
+          const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS, at = kb + lane * p.box;
+          const bool want = lane * p.box < CH_KEYS && at < it.t.hi;
+          // boxes below the window hold the first visible one in their place: their blocks may be gone
+          const int t = max(at, it.t.lo & -p.box);
           int blk = 0, b = 0;
           if (want) {
             b = t / g.bs;
@@ -1148,8 +1150,9 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
           if (warp == 9) {
             if (!(ok = mbar_wait(bar(BAR_RAWE + slot), phase ^ 1, abort_flag, err))) break;
-            const int t = kb + lane * p.box;
-            const bool want = lane * p.box < CH_KEYS && t < it.t.hi;
+            const int at = kb + lane * p.box;
+            const bool want = lane * p.box < CH_KEYS && at < it.t.hi;
+            const int t = max(at, it.t.lo & -p.box);  // as in the TMA loads
             int blk = 0, r = 0;
             if (want) {
               const int b = t / g.bs;
@@ -1235,6 +1238,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         const int u0 = qw * 32 + lane;
         const uint32_t raw_meta = sb + S::RAW + depth * UNITS * 16;
         auto key_of = [&](int j, int y) { return (it.t.k_lo + it.k0 + j) * CH_KEYS + (u0 + y * 7 * 32) / UPR; };
+        auto seen = [&](int key) { return key >= it.t.lo && key < it.t.hi; };  // the others are zeros
         // block ids (-1: no row) and rows in them of a load's units, a load ahead of the units themselves
         auto fetch_ids = [&](int i, int32_t (&blk)[N], int32_t (&row)[N]) {
           int j, kv;
@@ -1250,7 +1254,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
           for (int y = 0; y < N; ++y) {
             blk[y] = -1;
-            if (u0 + y * 7 * 32 < UNITS && key_of(j, y) < it.t.hi) blk[y] = __ldg(btrow + b[y]);
+            if (u0 + y * 7 * 32 < UNITS && seen(key_of(j, y))) blk[y] = __ldg(btrow + b[y]);
           }
         };
         // straight-line, so that the units' address arithmetic overlaps
@@ -1262,7 +1266,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
           for (int y = 0; y < N; ++y) {
             const int u = u0 + y * 7 * 32;
-            const bool unit = u < UNITS, want = unit && key_of(j, y) < it.t.hi;
+            const bool unit = u < UNITS, want = unit && seen(key_of(j, y));
             const bool good = want && (uint32_t)blk[y] < (uint32_t)g.nblocks;  // else zeros
             bad |= want && !good;
             const uint8_t* tile = base + (good ? blk[y] : 0) * block_bytes;
@@ -1296,7 +1300,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             if (!decltype(one)::value) {
               const int t = key_of(j, y);
               const int b = a.bs_log2 >= 0 ? t >> a.bs_log2 : t / g.bs;
-              const int32_t blk = t < it.t.hi ? __ldg(btrow + b) : -1;
+              const int32_t blk = seen(t) ? __ldg(btrow + b) : -1;
               if (blk >= 0 && blk < g.nblocks)
                 meta = head_base + (kv ? (int64_t)g.heads * g.tile_bytes : 0) + blk * block_bytes + g.bs * g.row_bytes +
                        (t - b * g.bs) * g.meta_row_bytes;

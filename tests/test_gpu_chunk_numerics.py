@@ -225,6 +225,30 @@ def test_tiny_keys_under_large_queries(cuda, dt, kscale, qscale):
     check_rows(pool, q, G, bt, [n], [310], out, dt)
 
 
+@pytest.mark.parametrize("dt,bits,meta,bs,D", [(orc.BF16, 0, orc.F16, 16, 128), (orc.F16, 0, orc.F16, 64, 64), (orc.BF16, 0, orc.F16, 5, 64),
+                                               (orc.BF16, 8, orc.F16, 16, 128), (orc.BF16, 4, orc.F32, 32, 64), (orc.F16, 8, orc.F32, 5, 128),
+                                               (orc.BF16, 4, orc.F16, 1, 128)])
+def test_freed_blocks_below_the_window(cuda, dt, bits, meta, bs, D):
+    """Table entries of blocks that lie wholly below every token's window may be anything: they are not read."""
+    H, G, window = 2, 4, 100
+    g = torch.Generator("cuda").manual_seed(36)
+    q_lens, lens = [1, 9, 150], [1000, 333, 701]
+    N = sum(-(-n // bs) for n in lens)
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=32, meta_dtype=meta)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda").to(TORCH[dt]) for _ in range(2))
+    pool.append(k, v, torch.arange(N * bs, device="cuda", dtype=torch.int32), N * bs)
+    bt = tables(lens, bs, N, g)
+    q = torch.randn(sum(q_lens), H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    whole = attend(pool, q, G, bt, q_lens, lens, window=window)
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, q_lens, lens, whole, dt, window=window)
+    for s, (n, L) in enumerate(zip(q_lens, lens)):
+        bt[s, :max(L - n - window + 1, 0) // bs] = [-1, N, 2 ** 31 - 1][s]
+    out = attend(pool, q, G, bt, q_lens, lens, window=window)
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, q_lens, lens, out, dt, window=window)
+
+
 @pytest.mark.parametrize("dt,bits", [(orc.BF16, 0), (orc.F16, 0), (orc.BF16, 8)])
 @pytest.mark.parametrize("D,n,L", [(128, 60, 100), (128, 60, 2000), (64, 3, 20000)])
 def test_rows_computed_again_repeat(cuda, dt, bits, D, n, L):
