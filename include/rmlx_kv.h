@@ -304,6 +304,10 @@ RMLX_API rmlx_status rmlx_kv_pool_check(rmlx_kv_pool* p, int32_t* device_error);
  * pinned host memory, or the copy is not asynchronous.  No counterpart in
  * the reference crate, whose errors are synchronous panics. */
 RMLX_API rmlx_status rmlx_kv_pool_status_async(rmlx_kv_pool* p, int32_t* status, void* stream);
+/* The time after which a wait inside a kernel of this pool gives up (30 s at
+ * first), for launches made after the call: see rmlx_kv_chunk_attention, the
+ * one kernel with such waits.  seconds in (0, 1e6]. */
+RMLX_API rmlx_status rmlx_kv_pool_set_wait_limit(rmlx_kv_pool* p, double seconds);
 
 /* Synchronous copies between host memory and pool bytes
  * [offset, offset + nbytes) (raw byte images of the pool; the prompt-cache
@@ -435,7 +439,15 @@ RMLX_API rmlx_status rmlx_kv_decode_attention(rmlx_kv_pool* p, int32_t layer, co
  * 16) and writes nothing.  Block ids outside the pool, and a sequence of more
  * rows than block_table_stride blocks (or 2^30) hold, are flagged (bit 2); what
  * that sequence's out rows then hold is unspecified.  Waits inside the kernel
- * are bounded: one that runs out (about 30 s) is flagged (bit 32).
+ * are bounded (rmlx_kv_pool_set_wait_limit): one that runs out is flagged (bit
+ * 32), the launch ends, and what its out rows hold is unspecified; later
+ * launches are not affected.  Only rows that are computed again take long: NaN
+ * or infinities that their mask hides, or, in a quantised pool, K or V groups
+ * beyond 65504, or f32 scales with V groups below 1.2e-4 where a row's outputs
+ * are that small too or K groups below 1.2e-4 under large queries (head_dim *
+ * max |q| * softmax_scale above 8192).  Each costs about 100 ns a key where 32
+ * are done in turn: one such row in reach of every token makes a call some 75
+ * times as long, and 256 of them over 9 million keys reach 30 s.
  * Pools, head_dim and q_heads_per_kv as for rmlx_kv_decode_attention; any
  * block size.  A quantised pool's rows count as code * scale + zero, without
  * the gather's rounding to cfg.dtype.  workspace: rmlx_kv_chunk_attention_workspace_size bytes, not

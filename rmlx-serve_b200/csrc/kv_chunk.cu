@@ -30,6 +30,7 @@ struct ChunkArgs {
   int gs_log2, bits, mf32;
   int bs_log2;  // of the block size, -1 when it is no power of two
   float scale_log2;
+  uint64_t wait_ns;  // limit of a wait
 };
 
 // ---------------------------------------------------------------------------
@@ -717,6 +718,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
   const uint32_t tmem = *tmem_slot;
   ItemIter it = *plan;
   const int qheads = g.heads * a.G;
+  uint32_t copies = 0;  // TMA or bulk loads that this warp has issued
 
   if (warp < 8) {
     // ---- softmax warpgroups -----------------------------------------------
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       bool ok = true;
       for (int j = 0; j < mine; ++j) {
         const int b = j & 1;
-        if (b == 0 && !(ok = mbar_wait(bar(BAR_S + x), ns++ & 1, abort_flag, err))) break;
+        if (b == 0 && !(ok = mbar_wait(bar(BAR_S + x), ns++ & 1, abort_flag, a.wait_ns, err))) break;
         if (active) {
           tc_fence_after();
           if (BITS && j == 0) c = a.scale_log2 * __uint_as_float((uint32_t)qscale[(nitem & 1) * CH_ROWS + row] << 23);
@@ -789,7 +791,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             if (j > 0) {
               // products into O have to be done: those of earlier tiles are (these scores were issued
               // behind them), the tile's first half signals its own
-              if (b && !(ok = mbar_wait(bar(BAR_V + x), (ns - 1) & 1, abort_flag, err))) break;
+              if (b && !(ok = mbar_wait(bar(BAR_V + x), (ns - 1) & 1, abort_flag, a.wait_ns, err))) break;
               tc_fence_after();
 #pragma unroll 1
               for (int i = 0; i < HD; i += 16) {
@@ -826,13 +828,13 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       const bool has[2] = {true, two || nk > 1};  // A and B have tiles
       if (!two) {
         if (x == 1) {
-          if (nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, abort_flag, err))) break;
+          if (nitem > 0 && !(ok = mbar_wait(bar(BAR_OFREE), (nitem - 1) & 1, abort_flag, a.wait_ns, err))) break;
           ml_b[wq * 32 + lane] = make_float2(ml, l);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(BAR_ML));
           writes = false;
         } else {
-          if (!(ok = mbar_wait(bar(BAR_ML), nml & 1, abort_flag, err))) break;
+          if (!(ok = mbar_wait(bar(BAR_ML), nml & 1, abort_flag, a.wait_ns, err))) break;
           const float2 b = ml_b[wq * 32 + lane];
           const float n = fmaxf(ml, b.x);
           const float base = n == -INFINITY ? 0.0f : n;
@@ -846,7 +848,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
       for (int y = 0; y < 2 && ok; ++y) {
         // a warpgroup reads its own O, and A reads B's too when they share rows
-        if (has[y] && (y == x || (!two && x == 0))) ok = mbar_wait(bar(BAR_O + y), no[y] & 1, abort_flag, err);
+        if (has[y] && (y == x || (!two && x == 0))) ok = mbar_wait(bar(BAR_O + y), no[y] & 1, abort_flag, a.wait_ns, err);
         no[y] += has[y];
       }
       if (!ok) break;
@@ -931,7 +933,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     uint32_t nitem = 0, pp = 0;  // items; a phase bit for each P buffer
     uint32_t st = 0, ph = 0;     // the ring's next stage and its phase
     bool ok = true;
-    auto wait = [&](int b, uint32_t parity) { return ok = ok && mbar_wait(bar(b), parity & 1, abort_flag, err); };
+    auto wait = [&](int b, uint32_t parity) { return ok = ok && mbar_wait(bar(b), parity & 1, abort_flag, a.wait_ns, err); };
     auto advance = [&] {
       if (++st == ST) st = 0, ph ^= 1;
     };
@@ -1023,11 +1025,6 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       if (!ok) break;
       ++nitem;
     }
-    if (!ok) {  // leave no MMA in flight behind
-      tc_commit(bar(BAR_DRAIN));
-      for (int i = 0; i < 2000 && !mbar_try(bar(BAR_DRAIN), 0); ++i) {
-      }
-    }
   } else {
     // ---- loads ----------------------------------------------------------------
     uint32_t n = 0, nitem = 0;
@@ -1042,7 +1039,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       const bool two = it.t.rows > 128;
       const int32_t* btrow = a.bt + (int64_t)it.s * a.bt_stride;
       if (loads_q) {
-        if (nitem > 0 && !(ok = mbar_wait(bar(BAR_QEMPTY), (nitem - 1) & 1, abort_flag, err))) break;
+        if (nitem > 0 && !(ok = mbar_wait(bar(BAR_QEMPTY), (nitem - 1) & 1, abort_flag, a.wait_ns, err))) break;
         constexpr int CPR = HD / 8, RPW = 32 / CPR;  // 16-byte chunks of a row, rows of a warp's pass
         const uint8_t* qbase = a.q + (int64_t)(it.qoff + it.t.t0) * a.qts + (int64_t)it.head * a.G * a.qhs;
         const int ch = lane % CPR;
@@ -1108,7 +1105,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           int j, kv;
           which(i, j, kv);
           const uint32_t stage = n % ST, dst = sb + S::KV + stage * S::STAGE;
-          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
+          if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, a.wait_ns, err))) break;
           ++n;
           // one box of p.box rows a lane
           const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS, at = kb + lane * p.box;
@@ -1149,7 +1146,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           const uint32_t slot = n % depth, phase = (n / depth) & 1, dst = sb + S::RAW + slot * raw_tile;
           const int kb = (it.t.k_lo + it.k0 + j) * CH_KEYS;
           if (warp == 9) {
-            if (!(ok = mbar_wait(bar(BAR_RAWE + slot), phase ^ 1, abort_flag, err))) break;
+            if (!(ok = mbar_wait(bar(BAR_RAWE + slot), phase ^ 1, abort_flag, a.wait_ns, err))) break;
             const int at = kb + lane * p.box;
             const bool want = lane * p.box < CH_KEYS && at < it.t.hi;
             const int t = max(at, it.t.lo & -p.box);  // as in the TMA loads
@@ -1172,9 +1169,9 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
               bulk_load(dst + CH_KEYS * RB + lane * p.box * mb, tile + g.bs * RB + r * mb, p.box * mb, bar(BAR_RAWF + slot));
             }
           } else {
-            if (!(ok = mbar_wait(bar(BAR_RAWF + slot), phase, abort_flag, err))) break;
+            if (!(ok = mbar_wait(bar(BAR_RAWF + slot), phase, abort_flag, a.wait_ns, err))) break;
             const uint32_t stage = n % ST, out = sb + S::KV + stage * S::STAGE;
-            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, err))) break;
+            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, a.wait_ns, err))) break;
             const int ch = lane % UPR;
             auto convert = [&](auto mf32, auto one) {  // f32 scales and zeros; a unit's elements are all of one group
               constexpr bool MF32 = decltype(mf32)::value;
@@ -1326,7 +1323,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           else if (one) convert_as(i, stage, slot, std::true_type(), std::true_type());
           else convert_as(i, stage, slot, std::true_type(), std::false_type());
         };
-        auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, abort_flag, err); };
+        auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, abort_flag, a.wait_ns, err); };
         int32_t ids[N], rows[N];
         fetch_ids(0, ids, rows);
         int in = 0, out = 0;  // ring slots of the next copy and the next conversion
@@ -1357,15 +1354,28 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       }
       if (!ok) break;
     }
-    if (issues && !ok) {  // leave no copy in flight behind
-      const uint32_t slots = raw ? p.raw_depth : ST;
-      for (uint32_t i = n > slots ? n - slots : 0; i < n; ++i)
-        for (int k = 0; k < 2000 && !mbar_try(bar((raw ? BAR_RAWF : BAR_FULL) + i % slots), (i / slots) & 1); ++k) {
-        }
-    }
+    if (issues) copies = n;
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    // A wait ran out, in whichever role: the others' MMAs and copies may still be in
+    // flight, and nothing may be when the CTA ends.
+    if (warp == 8) {
+      tc_commit(bar(BAR_DRAIN));
+      for (int i = 0; i < 2000 && !mbar_try(bar(BAR_DRAIN), 0); ++i) {
+      }
+    } else if (warp == 9) {
+      const uint32_t slots = raw ? p.raw_depth : ST;
+      for (uint32_t i = copies > slots ? copies - slots : 0; i < copies; ++i)
+        for (int k = 0; k < 2000 && !mbar_try(bar((raw ? BAR_RAWF : BAR_FULL) + i % slots), (i / slots) & 1); ++k) {
+        }
+    }
+    cp_async_wait_all();
+    if (threadIdx.x < 2) desc[threadIdx.x].valid = desc[threadIdx.x].last = 0;  // no part to join
+    tc_fence_before();
+    __syncthreads();
+  }
   if (warp == 8) tmem_free(tmem, 512);
 }
 
@@ -1386,6 +1396,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(ChunkParams p, int n
     const unsigned last = __ballot_sync(0xffffffffu, c0 + lane < nparts && p.desc[2 * (c0 + lane)].last);
     if (last) n = c0 - blockIdx.x + __ffs(last);
   }
+  if (n == 0) return;  // its last part's CTA gave up
   const float* first = p.parts + (size_t)(2 * blockIdx.x + 1) * part_floats(HD);  // a CTA's slot 1; the others' slot 0
   auto part = [&](int i) { return i == 0 ? first : first + (size_t)(2 * i - 1) * part_floats(HD); };
   auto max_sum = [&](int i) {
@@ -1535,6 +1546,7 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   a.max_len = (int)std::min<int64_t>((int64_t)block_table_stride * c.block_size, 1 << 30);
   a.gs_log2 = c.quant_bits ? log2i(c.group_size) : 0, a.bits = c.quant_bits, a.mf32 = c.meta_dtype == RMLX_F32;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;  // log2(e)
+  a.wait_ns = p->wait_ns;
   DeviceGuard dg(p->device);
   const bool bf = c.dtype == RMLX_BF16;
   ChunkParams prm;

@@ -776,6 +776,13 @@ rmlx_status rmlx_kv_pool_status_async(rmlx_kv_pool* p, int32_t* status, void* st
       "read error word");
 }
 
+rmlx_status rmlx_kv_pool_set_wait_limit(rmlx_kv_pool* p, double seconds) {
+  if (!p) return fail(RMLX_E_BAD_ARG, "NULL pool");
+  if (!(seconds > 0.0) || seconds > 1e6) return fail(RMLX_E_BAD_ARG, "the limit must lie in (0, 1e6] seconds");
+  p->wait_ns = (uint64_t)(seconds * 1e9);
+  return RMLX_OK;
+}
+
 rmlx_status rmlx_kv_pool_read(rmlx_kv_pool* p, size_t offset, size_t nbytes, void* host_dst) {
   if (!p || (nbytes && !host_dst)) return fail(RMLX_E_BAD_ARG, "NULL pool or destination");
   if (offset > p->bytes || nbytes > p->bytes - offset) return fail(RMLX_E_RANGE, "read past the end of the pool");

@@ -110,6 +110,7 @@ struct rmlx_kv_pool {
   // The chunk attention's kernels (made ready once) and the pool as TMA sees it (a CUtensorMap).
   void *chunk_fn = nullptr, *chunk_combine_fn = nullptr;
   alignas(64) uint8_t chunk_map[128] = {};
+  uint64_t wait_ns = 30000000000ull;  // limit of a wait inside a kernel
   rmlx::PoolGeo geo() const {
     rmlx::PoolGeo g;
     g.base = base;

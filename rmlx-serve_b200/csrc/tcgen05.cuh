@@ -39,31 +39,34 @@ __device__ __forceinline__ uint64_t global_ns() {
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
 }
-// Waits until the phase of `parity` has completed, at most about 30 s (a warp
-// that computes NaN rows again over millions of keys takes seconds): a wait
-// that runs out, or that sees another thread's run out, returns false (and
-// flags the launch), so every role leaves its loop and the CTA ends.
-__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+// Waits until the phase of `parity` has completed, at most about limit_ns (a
+// warp that computes rows again takes 3 us for each key of them): a wait that
+// runs out, or that sees another thread's run out, returns false (and flags the
+// launch), so every role leaves its loop and the CTA ends.
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                               int32_t* err) {
   const uint64_t t0 = global_ns();
 #pragma unroll 1
   for (uint32_t i = 0; i < (1u << 28); ++i) {
     if (mbar_try(bar, parity)) return true;
-    if ((i & 15) == 15 && (*abort_flag || global_ns() - t0 > 30000000000ull)) break;
+    if (*abort_flag || global_ns() - t0 > limit_ns) break;
   }
   *abort_flag = 1;
   atomicOr(err, DEV_ERR_TIMEOUT);
   return false;
 }
 // The wait of one thread.
-__device__ __forceinline__ bool mbar_wait_thread(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+__device__ __forceinline__ bool mbar_wait_thread(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                                 int32_t* err) {
 #pragma unroll 1
   for (int i = 0; i < 16; ++i)
     if (mbar_try(bar, parity)) return true;
-  return mbar_wait_slow(bar, parity, abort_flag, err);
+  return mbar_wait_slow(bar, parity, abort_flag, limit_ns, err);
 }
 // The wait of a whole warp: all lanes get the same answer.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
-  return __all_sync(0xffffffffu, mbar_wait_thread(bar, parity, abort_flag, err));
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                          int32_t* err) {
+  return __all_sync(0xffffffffu, mbar_wait_thread(bar, parity, abort_flag, limit_ns, err));
 }
 
 // Makes this thread's shared-memory writes visible to the async proxy (TMA, tcgen05).

@@ -112,6 +112,11 @@ class KVPool:
         this call has completed."""
         check(lib.rmlx_kv_pool_status_async(self._h, _ptr(word), _stream(stream, self.device)))
 
+    def set_wait_limit(self, seconds: float) -> None:
+        """The time after which a wait inside a kernel (chunk_attention) gives
+        up and flags the launch, for launches made after this call."""
+        check(lib.rmlx_kv_pool_set_wait_limit(self._h, float(seconds)))
+
     def read(self, offset: int = 0, nbytes: Optional[int] = None):
         """Copy pool bytes [offset, offset+nbytes) to a new host numpy array."""
         import numpy as np
