@@ -32,6 +32,15 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
                : "l"(p));
   return r;
 }
+// The same for bytes that the kernel itself may write: the non-coherent path
+// is for memory that stays as it is while the kernel runs.
+__device__ __forceinline__ uint4 ld_stream_coherent(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
 // 16-byte store with the evict-first (streaming) policy: gathered rows are
 // consumed by the next kernel or copied out, not re-read by this one.
 __device__ __forceinline__ void st_stream(void* p, uint4 v) {

@@ -73,7 +73,7 @@ struct Raw8 {
   uint4 w[N];
   __device__ __forceinline__ void load(const uint8_t* p) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = ld_stream(p + 16 * i);
+    for (int i = 0; i < N; ++i) w[i] = ld_stream_coherent(p + 16 * i);  // q_out may be q
   }
   __device__ __forceinline__ void store(uint8_t* p) const {
 #pragma unroll
