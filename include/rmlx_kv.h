@@ -351,7 +351,8 @@ typedef struct rmlx_rope {
  * q starts at element t * q_token_stride + h * q_head_stride, of q_out and of
  * k / v likewise (element type = cfg.dtype; pointers and strides multiples of
  * 16 bytes), so rows inside one fused projection are read in place; q_out may
- * be q with q's strides, and must not overlap q in any other way.  q_heads = 0
+ * be q with q's strides (others are refused), and must not overlap q in any
+ * other way.  q_heads = 0
  * rotates keys only.  Every token's query rows are written; a negative slot
  * skips the token's K and V.  Slots named twice in one call leave either
  * token's row (or a mixture of their bytes).  Angles are reduced in f64 and

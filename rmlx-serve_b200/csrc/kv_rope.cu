@@ -281,6 +281,8 @@ extern "C" rmlx_status rmlx_kv_append_rope(rmlx_kv_pool* p, int32_t layer, const
     return fail(RMLX_E_BAD_ARG, "k/v pointers and strides must be 16-byte aligned");
   if (q_heads && (!aligned16(q) || !aligned16(q_out) || (a.qts % 16) || (a.qhs % 16) || (a.ots % 16) || (a.ohs % 16)))
     return fail(RMLX_E_BAD_ARG, "q/q_out pointers and strides must be 16-byte aligned");
+  if (q_heads && q == q_out && ((num_tokens > 1 && a.qts != a.ots) || (q_heads > 1 && a.qhs != a.ohs)))
+    return fail(RMLX_E_BAD_ARG, "q_out is q with other strides");
   a.slots = slot_mapping, a.pos = positions, a.axis = rope->pair_axis, a.inv = rope->inv_freq;
   a.pos_stride = position_axis_stride;
   a.half = rope->rotary_dim / 2, a.naxes = rope->num_axes;

@@ -156,15 +156,16 @@ class KVPool:
 
         Strides are in elements and default to contiguous [tokens][heads]
         [head_dim]; positions are int32 [num_axes][num_tokens].  `q_out` may
-        be `q` itself (with q's strides)."""
+        be `q` itself: its strides are q's then."""
         c = self.cfg
         dim = c.head_dim
         hs = dim if head_stride is None else head_stride
         ts = c.num_kv_heads * dim if token_stride is None else token_stride
         qhs = dim if q_head_stride is None else q_head_stride
         qts = q_heads * dim if q_token_stride is None else q_token_stride
-        ohs = dim if q_out_head_stride is None else q_out_head_stride
-        ots = q_heads * dim if q_out_token_stride is None else q_out_token_stride
+        in_place = q is not None and _ptr(q_out) == _ptr(q)
+        ohs = (qhs if in_place else dim) if q_out_head_stride is None else q_out_head_stride
+        ots = (qts if in_place else q_heads * dim) if q_out_token_stride is None else q_out_token_stride
         ps = num_tokens if position_axis_stride is None else position_axis_stride
         check(lib.rmlx_kv_append_rope(self._h, layer, C.byref(rope._c), _ptr(positions), ps, _ptr(q), q_heads, qts, qhs,
                                       _ptr(q_out), ots, ohs, _ptr(k), _ptr(v), ts, hs, _ptr(slot_mapping), num_tokens,
