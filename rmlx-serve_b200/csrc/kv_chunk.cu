@@ -11,6 +11,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <mutex>
 #include <numeric>
 #include <type_traits>
 
@@ -1567,15 +1568,19 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   prm.desc = reinterpret_cast<PartDesc*>(prm.parts + (size_t)p->num_sms * 2 * part_floats(c.head_dim));
   static_assert(sizeof(CUtensorMap) == sizeof(p->chunk_map), "tensor map");
   const size_t smem = c.head_dim == 128 ? chunk_smem<128>(c.quant_bits) : chunk_smem<64>(c.quant_bits);
-  if (!p->chunk_fn) {  // the first call of a pool
-    if (tma && (s = chunk_map(p, prm.box, reinterpret_cast<CUtensorMap*>(p->chunk_map))) != RMLX_OK) return s;
-    ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
-                                   : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
-    if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
-    p->chunk_fn = reinterpret_cast<void*>(fn);
-    p->chunk_combine_fn = reinterpret_cast<void*>(
-        c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
-                          : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>));
+  if (!__atomic_load_n(&p->chunk_fn, __ATOMIC_ACQUIRE)) {  // the first calls of a pool, from one thread or several
+    static std::mutex first;
+    std::lock_guard<std::mutex> lock(first);
+    if (!p->chunk_fn) {
+      if (tma && (s = chunk_map(p, prm.box, reinterpret_cast<CUtensorMap*>(p->chunk_map))) != RMLX_OK) return s;
+      ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
+                                     : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
+      if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
+      p->chunk_combine_fn = reinterpret_cast<void*>(
+          c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
+                            : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>));
+      __atomic_store_n(&p->chunk_fn, reinterpret_cast<void*>(fn), __ATOMIC_RELEASE);  // last: what it stands for is ready
+    }
   }
   ChunkFn fn = reinterpret_cast<ChunkFn>(p->chunk_fn);
   ChunkCombineFn fc = reinterpret_cast<ChunkCombineFn>(p->chunk_combine_fn);

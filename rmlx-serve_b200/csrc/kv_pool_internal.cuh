@@ -107,7 +107,7 @@ struct rmlx_kv_pool {
   void* attn_fn = nullptr;
   size_t attn_smem = 0;
   int64_t attn_target = 0;
-  // The chunk attention's kernels (made ready once) and the pool as TMA sees it (a CUtensorMap).
+  // The chunk attention's kernels and the pool as TMA sees it (a CUtensorMap), made ready once: chunk_fn is set last.
   void *chunk_fn = nullptr, *chunk_combine_fn = nullptr;
   alignas(64) uint8_t chunk_map[128] = {};
   uint64_t wait_ns = 30000000000ull;  // limit of a wait inside a kernel
