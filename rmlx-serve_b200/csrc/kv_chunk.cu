@@ -1488,6 +1488,9 @@ rmlx_status chunk_map(rmlx_kv_pool* p, int box, CUtensorMap* map) {
     return reinterpret_cast<EncodeFn>(f);
   }();
   if (!encode) return fail(RMLX_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  // a driver call needs the device's context bound to this thread, which may have made no CUDA call before
+  const rmlx_status s = cuda_check(cudaSetDevice(p->device), "cudaSetDevice");
+  if (s != RMLX_OK) return s;
   const rmlx_pool_config& c = p->cfg;
   const cuuint64_t hd = c.head_dim;
   const cuuint64_t dims[4] = {64, 8, hd / 64, (cuuint64_t)c.num_blocks * c.num_layers * 2 * c.num_kv_heads * (c.block_size / 8)};
