@@ -252,10 +252,11 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // shared memory; should a row's output come out NaN all the same, its warp
 // computes that row again from the pool, reading visible rows only.
 //
-// Quantised pools: codes are dequantised to f16 in shared memory and the
-// products run in f16 (11 bits; bf16's 8 would add more error than the codes),
-// a bf16 query row scaled by a power of two to f16's upper end.  Groups whose
-// values leave f16's range become NaN, and their rows take that path too.
+// Quantised pools: codes are dequantised to f16 in shared memory (K of f16 pools in
+// two parts, CH_SPLIT) and the products run in f16 (11 bits; bf16's 8 would add
+// more error than the codes), a query row scaled by a power of two to f16's upper
+// end.  Groups whose values leave f16's range become NaN, and their rows take that
+// path too, as do rows that groups of tiny values matter to.
 // Where a box of codes and of (scale, zero) rows is whole 16-byte pieces, one
 // warp fetches them by bulk copies (1-16 tokens over 4-bit pools of 1024-8192
 // rows 190 us, against 200 with copies by the converting warps).
@@ -270,15 +271,25 @@ struct ChunkParams {
   PartDesc* desc;
 };
 
-template <int HD, int BITS>
+// f16 pools over codes: K in two f16 parts, a stage each.  Their outputs have three
+// bits more than bf16 ones, and K in one part cost most of them (rows with
+// outliers: error 2.2 to 4 times that of the output's own rounding, with two parts
+// 1.3 to 1.5); bf16 outputs show none of it (1.02 to 1.1).  The second part costs
+// more than a half of the time again: 8-bit chunks 386 us instead of 230.
+template <int DT, int BITS>
+constexpr bool CH_SPLIT = BITS && DT == RMLX_F16;
+
+template <int HD, int BITS, bool SPLIT>
 struct ChunkSmem {
   static constexpr int QTILE = 128 * HD * 2;
   static constexpr int STAGE = CH_KEYS * HD * 2;
   // Quantised pools give two stages up for codes in flight (RAW): 3 tiles of
-  // 8-bit codes with f16 scales, or 4 of 4-bit codes.
-  static constexpr int STAGES = BITS ? (HD == 128 ? 3 : 6) : HD == 128 ? 5 : 8;
+  // 8-bit codes with f16 scales, or 4 of 4-bit codes.  A fourth stage beside 3 tiles
+  // of 4-bit codes serves K in two parts (1-16 tokens over 4-bit rows 343 -> 304 us).
+  static constexpr bool FOURTH = SPLIT && BITS == 4 && HD == 128;
+  static constexpr int STAGES = BITS ? (HD == 128 ? 3 + FOURTH : 6) : HD == 128 ? 5 : 8;
   static constexpr int UNITS = BITS ? CH_KEYS * HD * BITS / 128 : 0;  // of a tile
-  static constexpr int RAW_BYTES = BITS == 8 ? UNITS * 60 : UNITS * 96;
+  static constexpr int RAW_BYTES = BITS == 8 ? UNITS * 60 : FOURTH ? UNITS * 56 : UNITS * 96;
   static constexpr int Q = 0, KV = 2 * QTILE, RAW = KV + STAGES * STAGE, CTRL = RAW + RAW_BYTES;
   // control block: barriers, then the plan, (max, sum) of warpgroup B, query scales, items with tiny groups
   static constexpr int BARS = CTRL, PLAN = CTRL + 352, ML = PLAN + 128, QSCALE = ML + 1024, TINY = QSCALE + 512;
@@ -416,6 +427,20 @@ __device__ __forceinline__ uint4 dequant8(uint2 w, const Group<BITS>& g) {
       v = __hfma2(c, g.sc2, g.zr2);
     }
     o[i] = *reinterpret_cast<uint32_t*>(&v);
+  }
+  return r;
+}
+// What dequant8's f16 elements leave of the values, in f16: both together hold 22 bits of them, or 2^-25.
+template <int BITS>
+__device__ __forceinline__ uint4 dequant8_rest(uint2 w, const Group<BITS>& g, uint4 hi) {
+  uint4 r;
+  const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
+  uint32_t* o = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = __byte_perm(i < 2 ? w.x : w.y, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
+    const float2 c = __half22float2(__hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1024.0f, 1024.0f)));
+    o[i] = pack2<RMLX_F16>(fmaf(c.x, g.sc, g.zr) - unpack_lo<RMLX_F16>(h[i]), fmaf(c.y, g.sc, g.zr) - unpack_hi<RMLX_F16>(h[i]));
   }
   return r;
 }
@@ -659,7 +684,8 @@ __device__ __noinline__ void attend_rows_again(const ChunkParams& p, const Again
 template <int DT, int HD, int BITS, bool TMA>
 __global__ void __launch_bounds__(ch_threads(TMA), 1)
     chunk_attn_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map, int32_t* err) {
-  using S = ChunkSmem<HD, BITS>;
+  constexpr bool SPLIT = CH_SPLIT<DT, BITS>;
+  using S = ChunkSmem<HD, BITS, SPLIT>;
   constexpr int CT = BITS ? RMLX_F16 : DT;  // type of the products' operands
   constexpr int ST = S::STAGES;
   constexpr uint32_t IDESC_S = mma_idesc(CT == RMLX_BF16, 128, CH_KEYS, false);
@@ -942,9 +968,30 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     constexpr uint32_t HALF = CH_HALF * HD * 2 / 16;
     const uint64_t qd = smem_desc(sb + S::Q, 16, 1024), kd = smem_desc(sb + S::KV, 16, HD * 16),
                    vd = smem_desc(sb + S::KV, 1024, HD * 16);
-    auto scores = [&](int x, int qt, uint32_t stage) {  // S[x] = Q[qt] K^T
-      mma_ss_rows<HD>(tmem + TM_S + 128 * x, qd + (uint32_t)(qt * (S::QTILE / 16)), kd + stage * (S::STAGE / 16), IDESC_S);
+    struct KeyStages {
+      uint32_t hi, lo;
+    };
+    auto scores = [&](int x, int qt, KeyStages k) {  // S[x] = Q[qt] K^T
+      const uint64_t q = qd + (uint32_t)(qt * (S::QTILE / 16));
+      mma_ss_rows<HD>(tmem + TM_S + 128 * x, q, kd + k.hi * (S::STAGE / 16), IDESC_S, 0);
+      if (SPLIT) mma_ss_rows<HD>(tmem + TM_S + 128 * x, q, kd + k.lo * (S::STAGE / 16), IDESC_S, 1);
       tc_commit(bar(BAR_S + x));
+    };
+    auto next_stage = [&] {  // once it is full; the ring's next one after it
+      const uint32_t s = st;
+      wait(BAR_FULL + s, ph);
+      advance();
+      return s;
+    };
+    auto next_keys = [&] {
+      KeyStages k;
+      k.hi = next_stage();
+      k.lo = SPLIT ? next_stage() : k.hi;
+      return k;
+    };
+    auto free_keys = [&](KeyStages k) {
+      tc_commit(bar(BAR_EMPTY + k.hi));
+      if (SPLIT) tc_commit(bar(BAR_EMPTY + k.lo));
     };
     auto values = [&](int x, uint32_t stage, int h, int keys, bool first) {  // O[x] (+)= P[x][h] V
       const uint64_t v0 = vd + (stage * (S::STAGE / 16) + h * HALF);
@@ -979,26 +1026,25 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
       const int lead = two ? 1 : min(2, nk);
       if (!wait(BAR_QFULL, nitem)) break;
       for (int i = 0; i < lead; ++i) {
-        if (!wait(BAR_FULL + st, ph)) break;
+        const KeyStages k = next_keys();
+        if (!ok) break;
         tc_fence_after();
-        scores(two ? 0 : i, 0, st);
-        if (two) scores(1, 1, st);
-        tc_commit(bar(BAR_EMPTY + st));
-        advance();
+        scores(two ? 0 : i, 0, k);
+        if (two) scores(1, 1, k);
+        free_keys(k);
       }
       if (!ok) break;
       if (lead == nk) tc_commit(bar(BAR_QEMPTY));
       if (nitem > 0 && !wait(BAR_OFREE, nitem - 1)) break;
       for (int j = 0; j < nk; ++j) {
-        const uint32_t sv = st;
-        if (!wait(BAR_FULL + sv, ph)) break;
-        advance();
+        const uint32_t sv = next_stage();
+        if (!ok) break;
         const int keys = keys_of(j), jn = j + lead;
         fill(sv, keys);
-        const uint32_t sk = st;
+        KeyStages sk = {0, 0};
         if (jn < nk) {
-          if (!wait(BAR_FULL + sk, ph)) break;
-          advance();
+          sk = next_keys();
+          if (!ok) break;
         }
         for (int y = 0; y < (two ? 2 : 1); ++y) {
           const int x = two ? y : j & 1;
@@ -1019,7 +1065,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         if (!ok) break;
         tc_commit(bar(BAR_EMPTY + sv));
         if (jn < nk) {
-          tc_commit(bar(BAR_EMPTY + sk));
+          free_keys(sk);
           if (jn == nk - 1) tc_commit(bar(BAR_QEMPTY));
         }
       }
@@ -1028,7 +1074,8 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
     }
   } else {
     // ---- loads ----------------------------------------------------------------
-    uint32_t n = 0, nitem = 0;
+    uint32_t n = 0, nitem = 0;   // loads, items
+    uint32_t ns = 0;             // stages filled (elsewhere than in SPLIT kernels a load is a stage)
     bool ok = true;
     const bool issues = (TMA || raw) && warp == 9, loads_q = !issues;
     const bool loads_kv = issues || !TMA;
@@ -1171,8 +1218,13 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             }
           } else {
             if (!(ok = mbar_wait(bar(BAR_RAWF + slot), phase, abort_flag, a.wait_ns, err))) break;
-            const uint32_t stage = n % ST, out = sb + S::KV + stage * S::STAGE;
-            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((n / ST) & 1) ^ 1, abort_flag, a.wait_ns, err))) break;
+            const bool both = SPLIT && kv == 0;
+            if (!SPLIT) ns = n;
+            const uint32_t stage = ns % ST, rest = (ns + 1) % ST;
+            const uint32_t out = sb + S::KV + stage * S::STAGE, out2 = sb + S::KV + rest * S::STAGE;
+            if (!(ok = mbar_wait(bar(BAR_EMPTY + stage), ((ns / ST) & 1) ^ 1, abort_flag, a.wait_ns, err))) break;
+            if (both && !(ok = mbar_wait(bar(BAR_EMPTY + rest), (((ns + 1) / ST) & 1) ^ 1, abort_flag, a.wait_ns, err))) break;
+            ns += both ? 2 : 1;
             const int ch = lane % UPR;
             auto convert = [&](auto mf32, auto one) {  // f32 scales and zeros; a unit's elements are all of one group
               constexpr bool MF32 = decltype(mf32)::value;
@@ -1202,8 +1254,9 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
 #pragma unroll
                 for (int e = 0; e < EPU / 8; ++e) {
                   if (!decltype(one)::value && e > 0) small |= grp.set(live ? pair(y, 8 * e) : make_uint2(0u, 0u), MF32);
-                  o[e] = dequant8<BITS ? BITS : 8, MF32>(
-                      BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
+                  const uint2 codes = BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]);
+                  o[e] = dequant8<BITS ? BITS : 8, MF32>(codes, grp);
+                  if (both) sts128(out2 + kv_off<HD>(row, ch * (EPU / 8) + e), dequant8_rest(codes, grp, o[e]));
                 }
 #pragma unroll
                 for (int e = 0; e < EPU / 8; ++e) sts128(out + kv_off<HD>(row, ch * (EPU / 8) + e), o[e]);
@@ -1217,7 +1270,11 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             else convert(std::true_type(), std::false_type());
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(BAR_FULL + stage)), mbar_arrive(bar(BAR_RAWE + slot));
+            if (lane == 0) {
+              mbar_arrive(bar(BAR_FULL + stage));
+              if (both) mbar_arrive(bar(BAR_FULL + rest));
+              mbar_arrive(bar(BAR_RAWE + slot));
+            }
           }
           ++n;
         }
@@ -1229,7 +1286,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
         // instead of the ring one tile was in flight: 4-bit chunks 290 us).
         constexpr int EPU = BITS ? 128 / (BITS ? BITS : 1) : 8, UPR = HD / EPU, UNITS = CH_KEYS * UPR;
         constexpr int N = (UNITS + 32 * 7 - 1) / (32 * 7);
-        const int depth = BITS == 0 ? 3 : BITS == 4 ? 4 : a.mf32 ? 2 : 3;
+        const int depth = BITS == 0 ? 3 : S::FOURTH ? 2 : BITS == 4 ? 4 : a.mf32 ? 2 : 3;
         const int ch = lane % UPR;  // the same for all of a lane's units
         const int64_t block_bytes = (int64_t)g.layers * 2 * g.heads * g.tile_bytes;
         const uint8_t* head_base = g.base + g.tile_off(0, a.layer, 0, it.head);
@@ -1280,7 +1337,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           }
         };
         // mf32: f32 scales and zeros; one: a unit's elements are all of one group
-        auto convert_as = [&](int i, uint32_t stage, int slot, auto mf32, auto one) {
+        auto convert_as = [&](int i, uint32_t stage, uint32_t rest, int slot, auto mf32, auto one) {
           constexpr bool MF32 = decltype(mf32)::value;
           int j, kv;
           which(i, j, kv);
@@ -1308,8 +1365,10 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
             for (int e = 0; e < EPU / 8; ++e) {
               if (!decltype(one)::value && e > 0 && meta)
                 small |= grp.set(load_meta(meta, (ch * EPU + 8 * e) >> a.gs_log2, MF32), MF32);
-              o[e] = dequant8<BITS ? BITS : 8, MF32>(
-                  BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]), grp);
+              const uint2 codes = BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]);
+              o[e] = dequant8<BITS ? BITS : 8, MF32>(codes, grp);
+              if (SPLIT && kv == 0)
+                sts128(sb + S::KV + rest * S::STAGE + kv_off<HD>(u / UPR, ch * (EPU / 8) + e), dequant8_rest(codes, grp, o[e]));
             }
 #pragma unroll
             for (int e = 0; e < EPU / 8; ++e)
@@ -1317,12 +1376,12 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           }
           if (MF32 && small) tiny[8 * kv + ((nitem - 1) & 7)] = nitem;
         };
-        auto convert = [&](int i, uint32_t stage, int slot) {
+        auto convert = [&](int i, uint32_t stage, uint32_t rest, int slot) {
           const bool one = (1 << a.gs_log2) >= EPU;
-          if (!a.mf32 && one) convert_as(i, stage, slot, std::false_type(), std::true_type());
-          else if (!a.mf32) convert_as(i, stage, slot, std::false_type(), std::false_type());
-          else if (one) convert_as(i, stage, slot, std::true_type(), std::true_type());
-          else convert_as(i, stage, slot, std::true_type(), std::false_type());
+          if (!a.mf32 && one) convert_as(i, stage, rest, slot, std::false_type(), std::true_type());
+          else if (!a.mf32) convert_as(i, stage, rest, slot, std::false_type(), std::false_type());
+          else if (one) convert_as(i, stage, rest, slot, std::true_type(), std::true_type());
+          else convert_as(i, stage, rest, slot, std::true_type(), std::false_type());
         };
         auto empty = [&](uint32_t i) { return ok = mbar_wait(bar(BAR_EMPTY + i % ST), ((i / ST) & 1) ^ 1, abort_flag, a.wait_ns, err); };
         int32_t ids[N], rows[N];
@@ -1341,14 +1400,26 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
           if (depth == 2) cp_async_wait<1>();
           else if (depth == 3) cp_async_wait<2>();
           else cp_async_wait<3>();
-          if (BITS != 0) {
-            if (!empty(n + d)) break;
-            convert(d, (n + d) % ST, out);
+          if constexpr (BITS != 0) {
+            int j, kv;
+            which(d, j, kv);
+            const bool both = SPLIT && kv == 0;
+            if (!SPLIT) ns = n + d;
+            if (!empty(ns) || (both && !empty(ns + 1))) break;
+            convert(d, ns % ST, (ns + 1) % ST, out);
             if (++out == depth) out = 0;
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(bar(BAR_FULL + ns % ST));
+              if (both) mbar_arrive(bar(BAR_FULL + (ns + 1) % ST));
+            }
+            ns += both ? 2 : 1;
+          } else {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(BAR_FULL + (n + d) % ST));
           }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(BAR_FULL + (n + d) % ST));
         }
         n += loads;
         if (bad) atomicOr(err, DEV_ERR_BLOCK);
@@ -1458,14 +1529,18 @@ ChunkFn pick_chunk(int bits, bool tma) {
   return tma ? chunk_attn_kernel<DT, HD, 0, true> : chunk_attn_kernel<DT, HD, 0, false>;
 }
 
-template <int HD>
-size_t chunk_smem(int bits) {
-  return bits == 8 ? ChunkSmem<HD, 8>::BYTES : bits == 4 ? ChunkSmem<HD, 4>::BYTES : ChunkSmem<HD, 0>::BYTES;
-}
-
-template <int HD>
-int chunk_raw(int bits) {
-  return bits == 8 ? ChunkSmem<HD, 8>::RAW_BYTES : ChunkSmem<HD, 4>::RAW_BYTES;
+// Shared memory of a launch, and what of it holds codes in flight.
+struct ChunkBytes {
+  size_t smem;
+  int raw;
+};
+template <int HD, bool F16>
+ChunkBytes chunk_bytes(int bits) {
+  using S8 = ChunkSmem<HD, 8, F16>;
+  using S4 = ChunkSmem<HD, 4, F16>;
+  if (bits == 8) return {S8::BYTES, S8::RAW_BYTES};
+  if (bits == 4) return {S4::BYTES, S4::RAW_BYTES};
+  return {ChunkSmem<HD, 0, false>::BYTES, 0};
 }
 
 size_t chunk_workspace(const rmlx_kv_pool* p) {
@@ -1560,17 +1635,17 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   // TMA reads whole groups of 8 stored rows; a box is the most rows that both a block and a key tile hold a whole number of
   prm.box = std::gcd(c.block_size, CH_KEYS);
   const bool tma = !c.quant_bits && c.block_size % 8 == 0;
+  const ChunkBytes bytes = c.head_dim == 128 ? (bf ? chunk_bytes<128, false>(c.quant_bits) : chunk_bytes<128, true>(c.quant_bits))
+                                             : (bf ? chunk_bytes<64, false>(c.quant_bits) : chunk_bytes<64, true>(c.quant_bits));
   // codes and their (scale, zero) rows by bulk copies where a box of either is whole 16-byte pieces (and 32 lanes issue a tile's)
   prm.raw_depth = 0;
   if (c.quant_bits && prm.box >= 4 && prm.box * p->meta_row_bytes % 16 == 0) {
-    const int room = c.head_dim == 128 ? chunk_raw<128>(c.quant_bits) : chunk_raw<64>(c.quant_bits);
-    const int depth = std::min<int>(CH_RAW, room / (CH_KEYS * (int)(p->row_bytes + p->meta_row_bytes)));
+    const int depth = std::min<int>(CH_RAW, bytes.raw / (CH_KEYS * (int)(p->row_bytes + p->meta_row_bytes)));
     if (depth >= 2) prm.raw_depth = depth;
   }
   prm.parts = static_cast<float*>(workspace);
   prm.desc = reinterpret_cast<PartDesc*>(prm.parts + (size_t)p->num_sms * 2 * part_floats(c.head_dim));
   static_assert(sizeof(CUtensorMap) == sizeof(p->chunk_map), "tensor map");
-  const size_t smem = c.head_dim == 128 ? chunk_smem<128>(c.quant_bits) : chunk_smem<64>(c.quant_bits);
   if (!__atomic_load_n(&p->chunk_fn, __ATOMIC_ACQUIRE)) {  // the first calls of a pool, from one thread or several
     static std::mutex first;
     std::lock_guard<std::mutex> lock(first);
@@ -1578,7 +1653,7 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
       if (tma && (s = chunk_map(p, prm.box, reinterpret_cast<CUtensorMap*>(p->chunk_map))) != RMLX_OK) return s;
       ChunkFn fn = c.head_dim == 128 ? (bf ? pick_chunk<RMLX_BF16, 128>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 128>(c.quant_bits, tma))
                                      : (bf ? pick_chunk<RMLX_BF16, 64>(c.quant_bits, tma) : pick_chunk<RMLX_F16, 64>(c.quant_bits, tma));
-      if ((s = prepare_smem(fn, smem)) != RMLX_OK) return s;
+      if ((s = prepare_smem(fn, bytes.smem)) != RMLX_OK) return s;
       p->chunk_combine_fn = reinterpret_cast<void*>(
           c.head_dim == 128 ? (bf ? chunk_combine_kernel<RMLX_BF16, 128> : chunk_combine_kernel<RMLX_F16, 128>)
                             : (bf ? chunk_combine_kernel<RMLX_BF16, 64> : chunk_combine_kernel<RMLX_F16, 64>));
@@ -1587,7 +1662,7 @@ rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* 
   }
   ChunkFn fn = reinterpret_cast<ChunkFn>(p->chunk_fn);
   ChunkCombineFn fc = reinterpret_cast<ChunkCombineFn>(p->chunk_combine_fn);
-  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(ch_threads(tma)), smem, (cudaStream_t)stream, prm,
+  cudaError_t e = launch_pdl(fn, dim3(p->num_sms), dim3(ch_threads(tma)), bytes.smem, (cudaStream_t)stream, prm,
                              *reinterpret_cast<const CUtensorMap*>(p->chunk_map), p->err);
   if (e != cudaSuccess) return cuda_check(e, "chunk attention launch");
   e = launch_pdl(fc, dim3(p->num_sms, CH_ROWS / 32), dim3(256), 0, (cudaStream_t)stream, prm, (int)p->num_sms);

@@ -154,15 +154,15 @@ __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int m, int n, bool b
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// D[tmem] = A[smem] B[smem]^T over HD columns, both operands contiguous along
+// D[tmem] (+)= A[smem] B[smem]^T over HD columns, both operands contiguous along
 // them in 64-column halves: 16 KB apart in A (128 rows), 1 KB apart in B (8 rows).
 template <int HD>
-__device__ __forceinline__ void mma_ss_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_ss_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if constexpr (HD == 128)
     asm volatile(
-        "{\n\t.reg .pred e, no, yes;\n\t.reg .b64 a, b;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 no, 0, 0;\n\tsetp.eq.u32 yes, 0, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, no;\n\t"
+        "{\n\t.reg .pred e, p, yes;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.eq.u32 yes, 0, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
         "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
         "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
@@ -177,20 +177,20 @@ __device__ __forceinline__ void mma_ss_rows(uint32_t d, uint64_t a, uint64_t b, 
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
         "add.s64 a, %1, 1030;\n\tadd.s64 b, %2, 70;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
-        "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc)
+        "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred e, no, yes;\n\t.reg .b64 a, b;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 no, 0, 0;\n\tsetp.eq.u32 yes, 0, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, no;\n\t"
+        "{\n\t.reg .pred e, p, yes;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.eq.u32 yes, 0, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
         "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
         "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
         "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, yes;\n\t"
-        "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc)
+        "}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem], 64 rows of B (HD columns each, 8 rows HD * 16 bytes apart).

@@ -308,3 +308,30 @@ def test_rows_computed_again_in_time(cuda, bits):
         assert pool.check() == 0
     assert torch.isfinite(out[:-1]).all() and torch.isnan(out[-1]).all()
     assert ms[1] <= 250 * ms[0], ms
+
+
+@pytest.mark.parametrize("bits,meta,gs,D,bs", [(8, orc.F16, 64, 128, 16), (4, orc.F16, 64, 128, 16), (8, orc.F32, 32, 64, 16),
+                                               (4, orc.F32, 64, 64, 5), (8, orc.F16, 8, 128, 1)])
+@pytest.mark.parametrize("n,L", [(70, 1500), (3, 9000)])
+def test_f16_pools_over_codes_lose_little(cuda, bits, meta, gs, D, bs, n, L):
+    """Rows with outliers in an f16 pool over codes: the error's norm against that of rounding the exact output to f16.
+    Weights, V and the output are rounded by half a step of f16 each, which in values of random sign are independent
+    shares of one size: sqrt(3) in all.  (With K in one f16 part its roundings alone came to 3.)"""
+    H, G, dt = 2, 4, orc.F16
+    g = torch.Generator("cuda").manual_seed(40 + D)
+    N = -(-L // bs)
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=gs, meta_dtype=meta)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda") for _ in range(2))
+    k, v = (torch.where(torch.rand(x.shape, generator=g, device="cuda") < 0.01, 8 * x, x).to(TORCH[dt]) for x in (k, v))
+    pool.append(k, v, torch.arange(N * bs, device="cuda", dtype=torch.int32), N * bs)
+    bt = torch.randperm(N, generator=g, device="cuda").to(torch.int32)[None]
+    q = torch.randn(n, H * G, D, generator=g, device="cuda").to(TORCH[dt])
+    out = attend(pool, q, G, bt, [n], [L])
+    assert pool.check() == 0
+    check_rows(pool, q, G, bt, [n], [L], out, dt)
+    kv = stored_rows(pool, 0, dt)[bt[0].long()]
+    kk, vv = (kv[:, i].transpose(0, 1).reshape(H, -1, D)[:, :L] for i in (0, 1))
+    s = torch.einsum("nhgd,hld->hgnl", q.double().view(n, H, G, D), kk) * D ** -0.5
+    hidden = torch.arange(L, device="cuda")[None] > torch.arange(L - n, L, device="cuda")[:, None]
+    want = torch.einsum("hgnl,hld->nhgd", torch.softmax(s.masked_fill(hidden, -np.inf), -1), vv).reshape(n, H * G, D)
+    assert (out.double() - want).norm() <= 2 * (want.half().double() - want).norm()
