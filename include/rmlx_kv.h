@@ -446,13 +446,20 @@ RMLX_API rmlx_status rmlx_kv_decode_attention(rmlx_kv_pool* p, int32_t layer, co
  * or infinities that their mask hides, or, in a quantised pool, K or V groups
  * beyond 65504, or f32 scales with V groups below 1.2e-4 where a row's outputs
  * are that small too or K groups below 1.2e-4 under large queries (head_dim *
- * max |q| * softmax_scale above 8192).  Each costs about 100 ns a key where 32
+ * max |q| * softmax_scale above 4096).  Each costs about 100 ns a key where 32
  * are done in turn: one such row in reach of every token makes a call some 75
  * times as long, and 256 of them over 9 million keys reach 30 s.
  * Pools, head_dim and q_heads_per_kv as for rmlx_kv_decode_attention; any
- * block size.  A quantised pool's rows count as code * scale + zero, without
- * the gather's rounding to cfg.dtype.  workspace: rmlx_kv_chunk_attention_workspace_size bytes, not
- * shared by launches that may overlap. */
+ * block size.  Rows are in the table's order, so the table of a ring
+ * (rmlx_rotating_*) serves until it wraps.
+ * A call repeated on the same GPU gives the same bits.  Scores, their maxima
+ * and sums and the output are f32 until the output's rounding.  Weights are
+ * rounded to bf16 in plain BF16 pools and otherwise to f16 (below 2^-21 of a
+ * row's largest by 2^-32 of it).  A quantised pool's rows count as code *
+ * scale + zero, without the gather's rounding to cfg.dtype; the products take
+ * them in f16 (11 bits, or 2^-25 where that is more), K of F16 pools in two
+ * parts (22 bits).  workspace: rmlx_kv_chunk_attention_workspace_size bytes,
+ * not shared by launches that may overlap. */
 RMLX_API rmlx_status rmlx_kv_chunk_attention_workspace_size(const rmlx_kv_pool* p, int32_t q_heads_per_kv,
                                                             size_t* bytes);
 RMLX_API rmlx_status rmlx_kv_chunk_attention(rmlx_kv_pool* p, int32_t layer, const void* q, int64_t q_token_stride,

@@ -239,8 +239,8 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // scores.  O is rescaled only when a row's maximum has grown by more than 2^8
 // since the last time (weights stay below 2^8, times the bias of f16; the final
 // division undoes both).
-// Measured for an 8192-token prompt (8 x 128, G = 4, bf16): 573 us, 960 TFLOP/s
-// of the causal work, in short bursts; 623 us at the power limit.  A key tile
+// Measured for an 8192-token prompt (8 x 128, G = 4, bf16): 559 us, 984 TFLOP/s
+// of the causal work, in bursts of 20 calls; 616 us at the power limit.  A key tile
 // takes a warpgroup about 2460 clocks of softmax and 1750 of waiting for the two
 // products, the tensor cores 2060.  Slower were: two threads a row (654 us), an
 // MMA warp for each warpgroup (726), weights through shared memory so that the
@@ -259,7 +259,7 @@ __host__ __device__ constexpr size_t part_floats(int hd) { return (size_t)CH_ROW
 // path too, as do rows that groups of tiny values matter to.
 // Where a box of codes and of (scale, zero) rows is whole 16-byte pieces, one
 // warp fetches them by bulk copies (1-16 tokens over 4-bit pools of 1024-8192
-// rows 190 us, against 200 with copies by the converting warps).
+// rows 184 us; with copies by the converting warps 10 us more).
 // ---------------------------------------------------------------------------
 struct ChunkParams {
   PoolGeo g;
