@@ -275,7 +275,7 @@ struct ChunkParams {
 // bits more than bf16 ones, and K in one part cost most of them (rows with
 // outliers: error 2.2 to 4 times that of the output's own rounding, with two parts
 // 1.3 to 1.5); bf16 outputs show none of it (1.02 to 1.1).  The second part costs
-// more than a half of the time again: 8-bit chunks 386 us instead of 230.
+// a half of the time again: 8-bit chunks 357 us instead of 230.
 template <int DT, int BITS>
 constexpr bool CH_SPLIT = BITS && DT == RMLX_F16;
 
@@ -285,7 +285,7 @@ struct ChunkSmem {
   static constexpr int STAGE = CH_KEYS * HD * 2;
   // Quantised pools give two stages up for codes in flight (RAW): 3 tiles of
   // 8-bit codes with f16 scales, or 4 of 4-bit codes.  A fourth stage beside 3 tiles
-  // of 4-bit codes serves K in two parts (1-16 tokens over 4-bit rows 343 -> 304 us).
+  // of 4-bit codes serves K in two parts (1-16 tokens over 4-bit rows 12 % shorter).
   static constexpr bool FOURTH = SPLIT && BITS == 4 && HD == 128;
   static constexpr int STAGES = BITS ? (HD == 128 ? 3 + FOURTH : 6) : HD == 128 ? 5 : 8;
   static constexpr int UNITS = BITS ? CH_KEYS * HD * BITS / 128 : 0;  // of a tile
@@ -323,7 +323,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 // Weights of a row's 64 scores: 2^(c s + nb), stored to TMEM in the products'
-// type, and their f32 sum.  All go to the special-function unit (4 a clock and
+// type (an MMA's operands have one 16-bit type; half a step of it costs about what
+// the output's own rounding does: error 1.2 to 1.4 times that of f32 weights), and
+// their f32 sum, of the unrounded ones.  All go to the special-function unit (4 a clock and
 // SM quarter): with 1/8 to 1/2 of them as polynomials on the FMA pipe the
 // softmax was shorter and the whole kernel slower (8192-token prompt 586 us,
 // with a quarter 624 us).
@@ -430,17 +432,34 @@ __device__ __forceinline__ uint4 dequant8(uint2 w, const Group<BITS>& g) {
   }
   return r;
 }
-// What dequant8's f16 elements leave of the values, in f16: both together hold 22 bits of them, or 2^-25.
-template <int BITS>
+// a b + c of f16 factors in f32, with one rounding.
+__device__ __forceinline__ float fma_f32_f16(__half a, __half b, float c) {
+  float d;
+  asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(__half_as_ushort(a)), "h"(__half_as_ushort(b)), "f"(c));
+  return d;
+}
+// What dequant8's f16 elements leave of the values, in f16: both together hold 22
+// bits of them, or 2^-25.  Mixed-precision multiply-adds take the f16 factors as
+// they are (with conversions of codes and elements to f32 8-bit chunks took 386 us).
+template <int BITS, bool MF32>
 __device__ __forceinline__ uint4 dequant8_rest(uint2 w, const Group<BITS>& g, uint4 hi) {
   uint4 r;
   const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
   uint32_t* o = reinterpret_cast<uint32_t*>(&r);
+  const __half minus = __ushort_as_half(0xbc00);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t m = __byte_perm(i < 2 ? w.x : w.y, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
-    const float2 c = __half22float2(__hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1024.0f, 1024.0f)));
-    o[i] = pack2<RMLX_F16>(fmaf(c.x, g.sc, g.zr) - unpack_lo<RMLX_F16>(h[i]), fmaf(c.y, g.sc, g.zr) - unpack_hi<RMLX_F16>(h[i]));
+    const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1024.0f, 1024.0f));
+    const __half2 x = *reinterpret_cast<const __half2*>(&h[i]);
+    float v0, v1;
+    if (MF32) {
+      const float2 f = __half22float2(c);
+      v0 = fmaf(f.x, g.sc, g.zr), v1 = fmaf(f.y, g.sc, g.zr);
+    } else {
+      v0 = fma_f32_f16(__low2half(c), __low2half(g.sc2), g.zr), v1 = fma_f32_f16(__high2half(c), __low2half(g.sc2), g.zr);
+    }
+    o[i] = pack2<RMLX_F16>(fma_f32_f16(__low2half(x), minus, v0), fma_f32_f16(__high2half(x), minus, v1));
   }
   return r;
 }
@@ -1256,7 +1275,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
                   if (!decltype(one)::value && e > 0) small |= grp.set(live ? pair(y, 8 * e) : make_uint2(0u, 0u), MF32);
                   const uint2 codes = BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]);
                   o[e] = dequant8<BITS ? BITS : 8, MF32>(codes, grp);
-                  if (both) sts128(out2 + kv_off<HD>(row, ch * (EPU / 8) + e), dequant8_rest(codes, grp, o[e]));
+                  if (both) sts128(out2 + kv_off<HD>(row, ch * (EPU / 8) + e), dequant8_rest<BITS ? BITS : 8, MF32>(codes, grp, o[e]));
                 }
 #pragma unroll
                 for (int e = 0; e < EPU / 8; ++e) sts128(out + kv_off<HD>(row, ch * (EPU / 8) + e), o[e]);
@@ -1368,7 +1387,7 @@ __global__ void __launch_bounds__(ch_threads(TMA), 1)
               const uint2 codes = BITS == 4 ? nibbles(cw[e & 3]) : make_uint2(cw[2 * (e & 1)], cw[2 * (e & 1) + 1]);
               o[e] = dequant8<BITS ? BITS : 8, MF32>(codes, grp);
               if (SPLIT && kv == 0)
-                sts128(sb + S::KV + rest * S::STAGE + kv_off<HD>(u / UPR, ch * (EPU / 8) + e), dequant8_rest(codes, grp, o[e]));
+                sts128(sb + S::KV + rest * S::STAGE + kv_off<HD>(u / UPR, ch * (EPU / 8) + e), dequant8_rest<BITS ? BITS : 8, MF32>(codes, grp, o[e]));
             }
 #pragma unroll
             for (int e = 0; e < EPU / 8; ++e)
