@@ -335,3 +335,24 @@ def test_f16_pools_over_codes_lose_little(cuda, bits, meta, gs, D, bs, n, L):
     hidden = torch.arange(L, device="cuda")[None] > torch.arange(L - n, L, device="cuda")[:, None]
     want = torch.einsum("hgnl,hld->nhgd", torch.softmax(s.masked_fill(hidden, -np.inf), -1), vv).reshape(n, H * G, D)
     assert (out.double() - want).norm() <= 2 * (want.half().double() - want).norm()
+
+
+@pytest.mark.parametrize("dt,bits,bs", [(orc.BF16, 0, 16), (orc.F16, 0, 5), (orc.BF16, 8, 16), (orc.F16, 4, 16)])
+def test_query_strides(cuda, dt, bits, bs):
+    """Queries laid out [head][token][dim], and one row for all tokens (stride 0): the bits of contiguous copies."""
+    H, G, D, n, L = 2, 4, 128, 150, 400
+    g = torch.Generator("cuda").manual_seed(41)
+    N = -(-L // bs)
+    pool = rmlx_kv.KVPool(1, H, D, bs, N, dtype=dt, quant_bits=bits, group_size=64, meta_dtype=orc.F16)
+    k, v = (torch.randn(N * bs, H, D, generator=g, device="cuda").to(TORCH[dt]) for _ in range(2))
+    pool.append(k, v, torch.arange(N * bs, device="cuda", dtype=torch.int32), N * bs)
+    bt = torch.arange(N, dtype=torch.int32, device="cuda")[None]
+    ws = torch.empty(pool.chunk_attention_workspace_size(G), dtype=torch.uint8, device="cuda")
+    by_head = torch.randn(H * G, n, D, generator=g, device="cuda").to(TORCH[dt])
+    for q, strides in ((by_head.transpose(0, 1), dict(q_token_stride=D, q_head_stride=n * D)),
+                       (by_head[:, :1].transpose(0, 1).expand(n, -1, -1), dict(q_token_stride=0, q_head_stride=n * D))):
+        out = torch.empty(n, H * G, D, dtype=TORCH[dt], device="cuda")
+        pool.chunk_attention(0, by_head, G, bt, N, dev([n]), dev([L]), 1, n, D ** -0.5, out, ws, **strides)
+        want = attend(pool, q.contiguous(), G, bt, [n], [L])
+        assert pool.check() == 0
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))
